@@ -50,6 +50,7 @@ extern "C" {
 #define NVFP4_STATUS_BAD_TAIL_ID 2u   /* tail length > 0 with a tail id outside [0, tail_pages) */
 #define NVFP4_STATUS_WAIT_TIMEOUT 4u  /* a bounded device-side wait gave up */
 #define NVFP4_STATUS_BAD_LENGTH 8u    /* seqused_fp4 not a multiple of 128 / beyond the table, tail length > 128 */
+#define NVFP4_STATUS_BAD_ROW 16u      /* page pool: a list names a row that does not exist, or one it must not name */
 
 /* decode implementations */
 #define NVFP4_IMPL_AUTO 0
@@ -519,6 +520,136 @@ int nvfp4_peer_merge(const float* const* o_part_ptrs, const float* const* lse_pa
  */
 int nvfp4_decode_host_io(const nvfp4_decode_args* args, const void* q_host, size_t q_bytes, void* out_host,
                          size_t out_bytes, void* stream);
+
+/*
+ * Chunks: several new tokens per row over the paged cache.  No counterpart in the reference, which
+ * serves whole prompts and single tokens only (src/nvfp4_vllm/guards.py:30-116 refuses the rest).
+ *
+ * The batch is ragged: row r's tokens are [chunk_start[r], chunk_start[r+1]) of the token buffers, 0 to
+ * max_chunk of them.  Its history is seqused_fp4[r] tokens in sealed NVFP4 pages (a multiple of 128)
+ * followed by seqused_tail[r] tokens (0 to 128) in BF16 tail page tail_ids[r].  All of these live on
+ * the device and nothing is read back; what is out of range is clamped, flagged in `status` and never
+ * made an address.  Buffers behind the last row's tokens are not touched.
+ */
+typedef struct nvfp4_chunk_args {
+  /* NVFP4 pages, as in nvfp4_decode_args */
+  void* k_packed;
+  int64_t k_pitch; /* bytes per page */
+  void* k_sf;
+  int64_t k_sf_pitch;
+  void* v_packed;
+  int64_t v_pitch;
+  void* v_sf;
+  int64_t v_sf_pitch;
+  int64_t num_pages;
+  const int32_t* page_table;      /* [rows][max_pages], row stride in elements */
+  int64_t page_table_row_stride;
+  int32_t max_pages;
+  const int32_t* seqused_fp4;     /* [rows] */
+  /* BF16 tail (all NULL/0 for an attention call whose rows have none) */
+  void* tail_key;                 /* [tail_pages][128][Hkv][128] bf16 */
+  void* tail_value;
+  int64_t tail_pages;
+  const int32_t* tail_ids;        /* [rows] */
+  const int32_t* seqused_tail;    /* [rows] */
+  /* the chunk */
+  const int32_t* chunk_start;     /* [rows + 1], ascending */
+  const void* key;                /* [tokens][Hkv][128] bf16, dense in a token, token strides in elements */
+  const void* value;
+  int64_t key_token_stride;
+  int64_t value_token_stride;
+  const void* key_shift;          /* nullable bf16 [Hkv][128]: subtracted from the chunk's keys (the cache holds shifted ones) */
+  int32_t rows;
+  int32_t tokens;                 /* tokens that the buffers hold */
+  int32_t max_chunk;              /* no row brings more tokens than this */
+  int32_t heads_kv;
+  uint32_t* status;               /* nullable sticky device status word */
+  /* attention only */
+  const void* query;              /* [tokens][Hq][128] bf16, strides in elements */
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  void* out;                      /* [tokens][Hq][128] bf16, dense in a token */
+  int64_t out_token_stride;
+  float* lse;                     /* nullable fp32 [tokens][Hq]: natural-log LSE of the scaled scores */
+  int32_t heads_q;
+  float softmax_scale;
+  int32_t num_splits;             /* >= 1: each row's keys in that many ranges, merged by a second launch */
+  void* workspace;                /* num_splits > 1: nvfp4_chunk_attention_workspace_bytes, 16-byte aligned */
+  size_t workspace_bytes;
+  /* append only: the lengths afterwards, in buffers of their own */
+  int32_t* seqused_fp4_out;       /* [rows] */
+  int32_t* seqused_tail_out;      /* [rows] */
+} nvfp4_chunk_args;
+
+/*
+ * Attention of the chunk's queries: token i of row r sees the row's whole history and the chunk's
+ * tokens 0..i.  Scores, softmax and sums in fp32; the pages' values enter as e2m1 * e4m3 exactly, the
+ * query and the chunk as BF16 - unlike nvfp4_decode, neither the query nor the probabilities are
+ * quantised to NVFP4.  The chunk's keys come from `key`, not from the cache: call it before (or
+ * after) nvfp4_append_chunk with the lengths from BEFORE the append, and before it whenever the
+ * append reuses the tail pages that this call reads.  Hq / Hkv: 1 to 8, 16 or 32.
+ */
+int nvfp4_chunk_attention(const nvfp4_chunk_args* args, void* stream);
+size_t nvfp4_chunk_attention_workspace_bytes(int tokens, int heads_q, int num_splits);
+
+/*
+ * Append the chunk to the cache: row r's stream is its tail followed by its (shifted) chunk; every
+ * full 128 tokens of it are quantised into the pages page_table[r][seqused_fp4[r]/128 ...] with the
+ * arithmetic of nvfp4_quantize_kv_pages, the remaining 0 to 127 tokens become the tail.  A row whose
+ * metadata is unusable (or whose table has no column left) keeps its cache and lengths and is flagged.
+ */
+int nvfp4_append_chunk(const nvfp4_chunk_args* args, void* stream);
+
+/*
+ * Pages back to BF16: key_out / value_out [count][128][Hkv][128] from pages page_ids[count] (e2m1 *
+ * e4m3, exact in BF16).  An id outside [0, num_pages) gives zeros and a flag.
+ */
+int nvfp4_dequantize_pages(const void* k_packed, int64_t k_pitch, const void* k_sf, int64_t k_sf_pitch,
+                           const void* v_packed, int64_t v_pitch, const void* v_sf, int64_t v_sf_pitch,
+                           int64_t num_pages, const int32_t* page_ids, int count, int heads_kv, void* key_out,
+                           void* value_out, uint32_t* status, void* stream);
+
+/*
+ * Page pool: pages that several rows share.  refs[page] counts the rows whose tables hold it; pages
+ * below `reserved` are never free and never moved.  Sealed pages are read-only, so a fork shares them
+ * and copies the BF16 tail alone.  No counterpart in the reference.
+ *
+ * release: for every row of `list` the first pages_held[row] entries of its table are given back
+ * and pages_held[row] becomes 0.  A row named twice is released once.
+ */
+int nvfp4_pool_release(const int32_t* list, int count, const int32_t* page_table, int64_t page_table_stride,
+                       int columns, int rows, int32_t* pages_held, int32_t* refs, int64_t num_pages,
+                       uint32_t* status, void* stream);
+/*
+ * fork: row targets[i] becomes a copy of row sources[i]: its first seqused_fp4/128 table entries (counted
+ * up), both lengths, and the tail (slot row_to_slot[target], every layer).  Pages that the source
+ * holds beyond its sealed ones are not shared.  Targets must hold nothing, be named once and be
+ * nobody's source; a pair that breaks one of the latter two is skipped and flagged.
+ */
+int nvfp4_pool_fork(const int32_t* sources, const int32_t* targets, int count, int32_t* page_table,
+                    int64_t page_table_stride, int columns, int rows, int32_t* pages_held, int32_t* seqused_fp4,
+                    int32_t* seqused_tail, const int32_t* row_to_slot, int32_t* refs, int64_t num_pages,
+                    void* tail_key, void* tail_value, int64_t layer_stride, int64_t slot_stride, int layers,
+                    int slots, int heads_kv, uint32_t* status, void* stream);
+/* ids [num_pages]: the free pages, ascending, then -1; count: how many. */
+int nvfp4_pool_free_list(const int32_t* refs, int64_t num_pages, int reserved, int32_t* ids, int32_t* count,
+                         void* stream);
+/*
+ * copy: page src[i] to page dst[i] in every layer; bases int64[layers] (device) are the layers' block
+ * arrays, pitch a block's bytes.  -1 in either list: nothing.  No page may be in both lists or twice in dst.
+ */
+int nvfp4_pool_copy(const int64_t* bases, int layers, int64_t pitch, int64_t num_pages, const int32_t* src,
+                    const int32_t* dst, int count, uint32_t* status, void* stream);
+/*
+ * compact: with L live pages (count > 0, or reserved), the k-th live page at or above L moves to the
+ * k-th free one below L, in every layer; counts move along and the first pages_held[row] entries of
+ * every row of the table are rewritten.  live_count: L.  workspace: nvfp4_pool_compact_workspace_bytes.
+ */
+int nvfp4_pool_compact(const int64_t* bases, int layers, int64_t pitch, int64_t num_pages, int reserved,
+                       int32_t* refs, int32_t* page_table, int64_t page_table_stride, int columns, int rows,
+                       const int32_t* pages_held, void* workspace, size_t workspace_bytes, int32_t* live_count,
+                       uint32_t* status, void* stream);
+size_t nvfp4_pool_compact_workspace_bytes(int64_t num_pages);
 
 #ifdef __cplusplus
 }

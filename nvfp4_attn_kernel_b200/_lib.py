@@ -20,7 +20,7 @@ DECODE_PERSISTENT = 4
 DECODE_WIDE_FORM = 8
 DECODE_MERGE_IN_LAUNCH = 16
 DECODE_HOST_IO_DIRECT = 32
-STATUS_BAD_PAGE_ID, STATUS_BAD_TAIL_ID, STATUS_WAIT_TIMEOUT, STATUS_BAD_LENGTH = 1, 2, 4, 8
+STATUS_BAD_PAGE_ID, STATUS_BAD_TAIL_ID, STATUS_WAIT_TIMEOUT, STATUS_BAD_LENGTH, STATUS_BAD_ROW = 1, 2, 4, 8, 16
 ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED = 1, 2, 3
 
 EXPORTS = (
@@ -55,6 +55,16 @@ EXPORTS = (
     "nvfp4_decode_persistent_workspace_bytes",
     "nvfp4_decode_persistent_supported",
     "nvfp4_decode_host_io",
+    "nvfp4_chunk_attention",
+    "nvfp4_chunk_attention_workspace_bytes",
+    "nvfp4_append_chunk",
+    "nvfp4_dequantize_pages",
+    "nvfp4_pool_release",
+    "nvfp4_pool_fork",
+    "nvfp4_pool_free_list",
+    "nvfp4_pool_copy",
+    "nvfp4_pool_compact",
+    "nvfp4_pool_compact_workspace_bytes",
 )
 
 
@@ -232,6 +242,83 @@ def _declare_static(lib) -> None:
     lib.nvfp4_decode_split_static_error.argtypes = []
 
 
+class ChunkArgs(ctypes.Structure):
+    """Mirror of ``struct nvfp4_chunk_args``."""
+
+    _fields_ = [
+        ("k_packed", c_void_p),
+        ("k_pitch", c_int64),
+        ("k_sf", c_void_p),
+        ("k_sf_pitch", c_int64),
+        ("v_packed", c_void_p),
+        ("v_pitch", c_int64),
+        ("v_sf", c_void_p),
+        ("v_sf_pitch", c_int64),
+        ("num_pages", c_int64),
+        ("page_table", c_void_p),
+        ("page_table_row_stride", c_int64),
+        ("max_pages", c_int32),
+        ("seqused_fp4", c_void_p),
+        ("tail_key", c_void_p),
+        ("tail_value", c_void_p),
+        ("tail_pages", c_int64),
+        ("tail_ids", c_void_p),
+        ("seqused_tail", c_void_p),
+        ("chunk_start", c_void_p),
+        ("key", c_void_p),
+        ("value", c_void_p),
+        ("key_token_stride", c_int64),
+        ("value_token_stride", c_int64),
+        ("key_shift", c_void_p),
+        ("rows", c_int32),
+        ("tokens", c_int32),
+        ("max_chunk", c_int32),
+        ("heads_kv", c_int32),
+        ("status", c_void_p),
+        ("query", c_void_p),
+        ("q_token_stride", c_int64),
+        ("q_head_stride", c_int64),
+        ("out", c_void_p),
+        ("out_token_stride", c_int64),
+        ("lse", c_void_p),
+        ("heads_q", c_int32),
+        ("softmax_scale", c_float),
+        ("num_splits", c_int32),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+        ("seqused_fp4_out", c_void_p),
+        ("seqused_tail_out", c_void_p),
+    ]
+
+
+def _declare_chunk(lib) -> None:
+    lib.nvfp4_chunk_attention.restype = c_int
+    lib.nvfp4_chunk_attention.argtypes = [ctypes.POINTER(ChunkArgs), c_void_p]
+    lib.nvfp4_chunk_attention_workspace_bytes.restype = c_size_t
+    lib.nvfp4_chunk_attention_workspace_bytes.argtypes = [c_int, c_int, c_int]
+    lib.nvfp4_append_chunk.restype = c_int
+    lib.nvfp4_append_chunk.argtypes = [ctypes.POINTER(ChunkArgs), c_void_p]
+    lib.nvfp4_dequantize_pages.restype = c_int
+    lib.nvfp4_dequantize_pages.argtypes = [c_void_p, c_int64] * 4 + [c_int64, c_void_p, c_int, c_int, c_void_p,
+                                                                     c_void_p, c_void_p, c_void_p]
+    lib.nvfp4_pool_release.restype = c_int
+    lib.nvfp4_pool_release.argtypes = [c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int64,
+                                       c_void_p, c_void_p]
+    lib.nvfp4_pool_fork.restype = c_int
+    lib.nvfp4_pool_fork.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int,
+                                    c_int, c_int, c_void_p, c_void_p]
+    lib.nvfp4_pool_free_list.restype = c_int
+    lib.nvfp4_pool_free_list.argtypes = [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]
+    lib.nvfp4_pool_copy.restype = c_int
+    lib.nvfp4_pool_copy.argtypes = [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p]
+    lib.nvfp4_pool_compact.restype = c_int
+    lib.nvfp4_pool_compact.argtypes = [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int,
+                                       c_int, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]
+    lib.nvfp4_pool_compact_workspace_bytes.restype = c_size_t
+    lib.nvfp4_pool_compact_workspace_bytes.argtypes = [c_int64]
+
+
 def load():
     """Load the shared library once and return the ctypes handle."""
     global _lib
@@ -247,6 +334,7 @@ def load():
         _declare_peer(lib)
         _declare_static(lib)
         _declare_control(lib)
+        _declare_chunk(lib)
         _lib = lib
     return _lib
 

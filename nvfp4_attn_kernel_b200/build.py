@@ -17,7 +17,7 @@ LIB_NAME = "libnvfp4_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 
 SOURCES = ["capi.cu", "quantize.cu", "decode_generic.cu", "decode_sm100.cu", "decode_persistent.cu", "merge.cu",
-           "decode_static_ws.cu", "control.cu", "key_sum.cu"]
+           "decode_static_ws.cu", "control.cu", "key_sum.cu", "chunk_attention.cu", "chunk_append.cu", "page_pool.cu"]
 # measurement aid of bench.py, a library of its own so that the product's ABI carries no test code
 BENCH_AID_SOURCE = "bench_read_floor.cu"
 BENCH_AID_PATH = os.path.join(HERE, "libnvfp4_bench_read_floor.so")

@@ -741,4 +741,221 @@ size_t nvfp4_push_merge_inbox_floats(int world, int rows, int heads_q) {
   return (size_t)2 * world * rows * heads_q * 132;
 }
 
+namespace {
+
+// The checks that the chunk entry points share; `tail` 0: must be absent or whole, 1: required.
+int chunk_cache(const nvfp4_chunk_args* a, const char* who, bool need_tail, nvfp4::ChunkCache* c) {
+  if (!a) return fail(NVFP4_ERR_INVALID, "%s: null argument block", who);
+  if (a->rows < 0 || a->tokens < 0 || a->max_chunk < 0) return fail(NVFP4_ERR_INVALID, "%s: negative extent", who);
+  if (a->rows > 65535) return fail(NVFP4_ERR_INVALID, "%s: too many rows: %d", who, a->rows);
+  if (a->heads_kv < 1 || a->heads_kv > 128)
+    return fail(NVFP4_ERR_INVALID, "%s: heads_kv out of range: %d", who, a->heads_kv);
+  if (a->max_pages < 0 || a->num_pages < 0 || a->num_pages > INT32_MAX)
+    return fail(NVFP4_ERR_INVALID, "%s: page counts out of range", who);
+  if (!a->seqused_fp4 || !a->chunk_start) return fail(NVFP4_ERR_INVALID, "%s: null lengths", who);
+  if (a->tokens > 0 && (!a->key || !a->value)) return fail(NVFP4_ERR_INVALID, "%s: key and value must be non-null", who);
+  const int64_t width = (int64_t)a->heads_kv * 128;
+  if (a->key_token_stride < width || a->value_token_stride < width || (a->key_token_stride % 8) ||
+      (a->value_token_stride % 8) || !aligned16(a->key) || !aligned16(a->value) || !aligned16(a->key_shift))
+    return fail(NVFP4_ERR_INVALID, "%s: key and value must be dense within a token and 16-byte aligned", who);
+  if (a->max_pages > 0) {
+    if (!a->page_table || !a->k_packed || !a->k_sf || !a->v_packed || !a->v_sf)
+      return fail(NVFP4_ERR_INVALID, "%s: page regions and table must be non-null", who);
+    if (a->page_table_row_stride < a->max_pages)
+      return fail(NVFP4_ERR_INVALID, "%s: page_table_row_stride is smaller than max_pages", who);
+    const int64_t packed = width * 64, sf = (int64_t)a->heads_kv * 1024;
+    if (a->k_pitch < packed || a->v_pitch < packed || a->k_sf_pitch < sf || a->v_sf_pitch < sf || (a->k_pitch % 16) ||
+        (a->v_pitch % 16) || (a->k_sf_pitch % 16) || (a->v_sf_pitch % 16) || !aligned16(a->k_packed) ||
+        !aligned16(a->k_sf) || !aligned16(a->v_packed) || !aligned16(a->v_sf))
+      return fail(NVFP4_ERR_INVALID, "%s: page regions need a page's bytes as pitch and 16-byte alignment", who);
+  }
+  const int given = !!a->tail_key + !!a->tail_value + !!a->tail_ids + !!a->seqused_tail;
+  if (given != 0 && given != 4) return fail(NVFP4_ERR_INVALID, "%s: the tail's four arguments go together", who);
+  if (need_tail && given == 0) return fail(NVFP4_ERR_INVALID, "%s: needs the BF16 tail", who);
+  if (given && (!aligned16(a->tail_key) || !aligned16(a->tail_value) || a->tail_pages < 0))
+    return fail(NVFP4_ERR_INVALID, "%s: tail pages must be 16-byte aligned", who);
+  *c = nvfp4::ChunkCache{};
+  c->k_packed = static_cast<uint8_t*>(a->k_packed); c->k_pitch = a->k_pitch;
+  c->k_sf = static_cast<uint8_t*>(a->k_sf); c->k_sf_pitch = a->k_sf_pitch;
+  c->v_packed = static_cast<uint8_t*>(a->v_packed); c->v_pitch = a->v_pitch;
+  c->v_sf = static_cast<uint8_t*>(a->v_sf); c->v_sf_pitch = a->v_sf_pitch;
+  c->num_pages = a->num_pages;
+  c->page_table = a->page_table; c->page_table_row_stride = a->page_table_row_stride; c->max_pages = a->max_pages;
+  c->seqused_fp4 = a->seqused_fp4;
+  c->tail_key = static_cast<uint16_t*>(a->tail_key); c->tail_value = static_cast<uint16_t*>(a->tail_value);
+  c->tail_pages = given ? a->tail_pages : 0;
+  c->tail_ids = a->tail_ids; c->seqused_tail = a->seqused_tail;
+  c->chunk_start = a->chunk_start;
+  c->key = static_cast<const uint16_t*>(a->key); c->value = static_cast<const uint16_t*>(a->value);
+  c->key_stride = a->key_token_stride; c->value_stride = a->value_token_stride;
+  c->key_shift = static_cast<const uint16_t*>(a->key_shift);
+  c->rows = a->rows; c->tokens = a->tokens; c->max_chunk = a->max_chunk; c->heads_kv = a->heads_kv;
+  c->status = a->status;
+  return NVFP4_OK;
+}
+
+}  // namespace
+
+size_t nvfp4_chunk_attention_workspace_bytes(int tokens, int heads_q, int num_splits) {
+  if (num_splits <= 1 || tokens < 1 || heads_q < 1) return 0;
+  return (size_t)num_splits * tokens * heads_q * (128 + 1) * sizeof(float);
+}
+
+int nvfp4_chunk_attention(const nvfp4_chunk_args* a, void* stream) {
+  nvfp4::ChunkAttention p{};
+  if (int code = chunk_cache(a, "chunk_attention", false, &p.c)) return code;
+  if (!valid_group(a->heads_q, a->heads_kv))
+    return fail(NVFP4_ERR_UNSUPPORTED, "chunk_attention: heads_q / heads_kv must be 1 to 8, 16 or 32 (%d, %d)",
+                a->heads_q, a->heads_kv);
+  if (!(a->softmax_scale > 0.f) || !(a->softmax_scale < 1e30f))
+    return fail(NVFP4_ERR_INVALID, "chunk_attention: softmax_scale must be finite and positive");
+  if (a->num_splits < 1 || a->num_splits > 128)
+    return fail(NVFP4_ERR_INVALID, "chunk_attention: num_splits must be 1 to 128, got %d", a->num_splits);
+  if (a->rows == 0 || a->tokens == 0 || a->max_chunk == 0) return NVFP4_OK;
+  if (!a->query || !a->out) return fail(NVFP4_ERR_INVALID, "chunk_attention: query and out must be non-null");
+  if (!aligned16(a->query) || !aligned16(a->out) || (a->q_token_stride % 8) || (a->q_head_stride % 8) ||
+      (a->out_token_stride % 8) || a->out_token_stride < (int64_t)a->heads_q * 128)
+    return fail(NVFP4_ERR_INVALID, "chunk_attention: query and out must keep 16-byte alignment, out dense in a token");
+  if (a->num_splits > 1) {
+    const size_t need = nvfp4_chunk_attention_workspace_bytes(a->tokens, a->heads_q, a->num_splits);
+    if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))
+      return fail(NVFP4_ERR_INVALID, "chunk_attention: needs a 16-byte aligned workspace of %zu bytes, got %zu", need,
+                  a->workspace_bytes);
+    p.o_partial = static_cast<float*>(a->workspace);
+    p.lse_partial = p.o_partial + (size_t)a->num_splits * a->tokens * a->heads_q * 128;
+  }
+  p.query = static_cast<const uint16_t*>(a->query);
+  p.q_token_stride = a->q_token_stride; p.q_head_stride = a->q_head_stride;
+  p.out = static_cast<uint16_t*>(a->out); p.out_token_stride = a->out_token_stride;
+  p.lse = a->lse; p.heads_q = a->heads_q; p.num_splits = a->num_splits;
+  p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  cudaError_t e = nvfp4::launch_chunk_attention(p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "chunk_attention launch");
+}
+
+int nvfp4_append_chunk(const nvfp4_chunk_args* a, void* stream) {
+  nvfp4::ChunkCache c;
+  if (int code = chunk_cache(a, "append_chunk", true, &c)) return code;
+  if (a->rows == 0) return NVFP4_OK;
+  if (!a->seqused_fp4_out || !a->seqused_tail_out)
+    return fail(NVFP4_ERR_INVALID, "append_chunk: the lengths afterwards need buffers");
+  if (a->seqused_fp4_out == a->seqused_fp4 || a->seqused_tail_out == a->seqused_tail ||
+      a->seqused_fp4_out == a->seqused_tail || a->seqused_tail_out == a->seqused_fp4)
+    return fail(NVFP4_ERR_INVALID, "append_chunk: the lengths afterwards need buffers of their own");
+  if (a->max_chunk / 128 + 2 > 65535) return fail(NVFP4_ERR_INVALID, "append_chunk: max_chunk too large");
+  cudaError_t e = nvfp4::launch_append_chunk(c, a->seqused_fp4_out, a->seqused_tail_out,
+                                             static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "append_chunk launch");
+}
+
+int nvfp4_dequantize_pages(const void* k_packed, int64_t k_pitch, const void* k_sf, int64_t k_sf_pitch,
+                           const void* v_packed, int64_t v_pitch, const void* v_sf, int64_t v_sf_pitch,
+                           int64_t num_pages, const int32_t* page_ids, int count, int heads_kv, void* key_out,
+                           void* value_out, uint32_t* status, void* stream) {
+  if (count < 0 || num_pages < 0) return fail(NVFP4_ERR_INVALID, "dequantize_pages: negative extent");
+  if (heads_kv < 1 || heads_kv > 128) return fail(NVFP4_ERR_INVALID, "dequantize_pages: heads_kv out of range: %d", heads_kv);
+  if (count == 0) return NVFP4_OK;
+  if (!k_packed || !k_sf || !v_packed || !v_sf || !page_ids || !key_out || !value_out)
+    return fail(NVFP4_ERR_INVALID, "dequantize_pages: null argument");
+  const int64_t packed = (int64_t)heads_kv * 8192, sf = (int64_t)heads_kv * 1024;
+  if (k_pitch < packed || v_pitch < packed || k_sf_pitch < sf || v_sf_pitch < sf || (k_pitch % 16) || (v_pitch % 16) ||
+      (k_sf_pitch % 16) || (v_sf_pitch % 16) || !aligned16(k_packed) || !aligned16(k_sf) || !aligned16(v_packed) ||
+      !aligned16(v_sf) || !aligned16(key_out) || !aligned16(value_out))
+    return fail(NVFP4_ERR_INVALID, "dequantize_pages: regions need a page's bytes as pitch and 16-byte alignment");
+  nvfp4::ChunkCache c{};
+  c.k_packed = static_cast<uint8_t*>(const_cast<void*>(k_packed)); c.k_pitch = k_pitch;
+  c.k_sf = static_cast<uint8_t*>(const_cast<void*>(k_sf)); c.k_sf_pitch = k_sf_pitch;
+  c.v_packed = static_cast<uint8_t*>(const_cast<void*>(v_packed)); c.v_pitch = v_pitch;
+  c.v_sf = static_cast<uint8_t*>(const_cast<void*>(v_sf)); c.v_sf_pitch = v_sf_pitch;
+  c.num_pages = num_pages; c.heads_kv = heads_kv; c.status = status;
+  cudaError_t e = nvfp4::launch_dequantize_pages(c, page_ids, count, key_out, value_out,
+                                                 static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "dequantize_pages launch");
+}
+
+int nvfp4_pool_release(const int32_t* list, int count, const int32_t* page_table, int64_t page_table_stride,
+                       int columns, int rows, int32_t* pages_held, int32_t* refs, int64_t num_pages,
+                       uint32_t* status, void* stream) {
+  if (count < 0 || rows < 0 || columns < 0 || num_pages < 0) return fail(NVFP4_ERR_INVALID, "pool_release: negative extent");
+  if (count == 0) return NVFP4_OK;
+  if (!list || !page_table || !pages_held || !refs) return fail(NVFP4_ERR_INVALID, "pool_release: null argument");
+  if (rows > 1 && page_table_stride < columns)
+    return fail(NVFP4_ERR_INVALID, "pool_release: page_table_stride is smaller than the table's columns");
+  cudaError_t e = nvfp4::launch_pool_release(list, count, page_table, page_table_stride, columns, rows, pages_held,
+                                             refs, num_pages, status, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "pool_release launch");
+}
+
+int nvfp4_pool_fork(const int32_t* sources, const int32_t* targets, int count, int32_t* page_table,
+                    int64_t page_table_stride, int columns, int rows, int32_t* pages_held, int32_t* seqused_fp4,
+                    int32_t* seqused_tail, const int32_t* row_to_slot, int32_t* refs, int64_t num_pages,
+                    void* tail_key, void* tail_value, int64_t layer_stride, int64_t slot_stride, int layers,
+                    int slots, int heads_kv, uint32_t* status, void* stream) {
+  if (count < 0 || rows < 0 || columns < 0 || num_pages < 0 || layers < 0 || slots < 0)
+    return fail(NVFP4_ERR_INVALID, "pool_fork: negative extent");
+  if (count == 0) return NVFP4_OK;
+  if (count > 65535) return fail(NVFP4_ERR_INVALID, "pool_fork: too many pairs: %d", count);
+  if (!sources || !targets || !page_table || !pages_held || !seqused_fp4 || !seqused_tail || !refs)
+    return fail(NVFP4_ERR_INVALID, "pool_fork: null argument");
+  if (rows > 1 && page_table_stride < columns)
+    return fail(NVFP4_ERR_INVALID, "pool_fork: page_table_stride is smaller than the table's columns");
+  if (layers > 0) {
+    if (!tail_key || !tail_value || !row_to_slot) return fail(NVFP4_ERR_INVALID, "pool_fork: null tail argument");
+    if (heads_kv < 1 || heads_kv > 128) return fail(NVFP4_ERR_INVALID, "pool_fork: heads_kv out of range: %d", heads_kv);
+    if (slot_stride < (int64_t)128 * 128 * heads_kv || (slot_stride % 8) || (layer_stride % 8) ||
+        !aligned16(tail_key) || !aligned16(tail_value) || layers > 1024)
+      return fail(NVFP4_ERR_INVALID, "pool_fork: tails need a slot's size as stride and 16-byte alignment, at most 1024 layers");
+  }
+  const nvfp4::PoolFork f{sources, targets, count, page_table, page_table_stride, columns, rows, pages_held, seqused_fp4,
+                          seqused_tail, row_to_slot, refs, num_pages, static_cast<uint16_t*>(tail_key),
+                          static_cast<uint16_t*>(tail_value), layer_stride, slot_stride, layers, slots, heads_kv, status};
+  cudaError_t e = nvfp4::launch_pool_fork(f, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "pool_fork launch");
+}
+
+int nvfp4_pool_free_list(const int32_t* refs, int64_t num_pages, int reserved, int32_t* ids, int32_t* count,
+                         void* stream) {
+  if (num_pages < 0 || num_pages > INT32_MAX || reserved < 0) return fail(NVFP4_ERR_INVALID, "pool_free_list: bad extent");
+  if (!count || (num_pages > 0 && (!refs || !ids))) return fail(NVFP4_ERR_INVALID, "pool_free_list: null argument");
+  cudaError_t e = nvfp4::launch_pool_free_list(refs, num_pages, reserved, ids, count, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "pool_free_list launch");
+}
+
+int nvfp4_pool_copy(const int64_t* bases, int layers, int64_t pitch, int64_t num_pages, const int32_t* src,
+                    const int32_t* dst, int count, uint32_t* status, void* stream) {
+  if (layers < 0 || count < 0 || num_pages < 0) return fail(NVFP4_ERR_INVALID, "pool_copy: negative extent");
+  if (count == 0 || layers == 0) return NVFP4_OK;
+  if (!bases || !src || !dst) return fail(NVFP4_ERR_INVALID, "pool_copy: null argument");
+  if (pitch < 16 || (pitch % 16)) return fail(NVFP4_ERR_INVALID, "pool_copy: a block must be a multiple of 16 bytes");
+  cudaError_t e = nvfp4::launch_pool_copy(bases, layers, pitch, num_pages, src, dst, count, status,
+                                          static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "pool_copy launch");
+}
+
+size_t nvfp4_pool_compact_workspace_bytes(int64_t num_pages) {
+  return num_pages < 0 ? 0 : (size_t)(3 * num_pages + 1) * sizeof(int32_t);
+}
+
+int nvfp4_pool_compact(const int64_t* bases, int layers, int64_t pitch, int64_t num_pages, int reserved,
+                       int32_t* refs, int32_t* page_table, int64_t page_table_stride, int columns, int rows,
+                       const int32_t* pages_held, void* workspace, size_t workspace_bytes, int32_t* live_count,
+                       uint32_t* status, void* stream) {
+  if (layers < 1 || num_pages < 1 || num_pages > INT32_MAX || reserved < 0 || columns < 0 || rows < 0 || rows > (1 << 20))
+    return fail(NVFP4_ERR_INVALID, "pool_compact: bad extent");
+  if (!bases || !refs || !live_count || (rows > 0 && (!page_table || !pages_held)))
+    return fail(NVFP4_ERR_INVALID, "pool_compact: null argument");
+  if (pitch < 16 || (pitch % 16)) return fail(NVFP4_ERR_INVALID, "pool_compact: a block must be a multiple of 16 bytes");
+  if (rows > 1 && page_table_stride < columns)
+    return fail(NVFP4_ERR_INVALID, "pool_compact: page_table_stride is smaller than the table's columns");
+  const size_t need = nvfp4_pool_compact_workspace_bytes(num_pages);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(NVFP4_ERR_INVALID, "pool_compact: needs a 16-byte aligned workspace of %zu bytes, got %zu", need,
+                workspace_bytes);
+  cudaError_t e = nvfp4::launch_pool_compact(bases, layers, pitch, num_pages, reserved, refs, page_table,
+                                             page_table_stride, columns, rows, pages_held,
+                                             static_cast<int32_t*>(workspace), live_count, status,
+                                             static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "pool_compact launch");
+}
+
 }  // extern "C"

@@ -177,4 +177,61 @@ cudaError_t launch_push_merge(const float* o_local, int64_t o_split_stride, cons
 cudaError_t launch_key_sum(const void* key, int64_t token_stride, int tokens, int heads_kv, double* sum,
                            cudaStream_t stream);
 
+// The paged cache and the ragged batch that the chunk kernels work on.
+struct ChunkCache {
+  uint8_t* k_packed; int64_t k_pitch;
+  uint8_t* k_sf; int64_t k_sf_pitch;
+  uint8_t* v_packed; int64_t v_pitch;
+  uint8_t* v_sf; int64_t v_sf_pitch;
+  int64_t num_pages;
+  const int32_t* page_table; int64_t page_table_row_stride; int max_pages;
+  const int32_t* seqused_fp4;
+  uint16_t* tail_key; uint16_t* tail_value; int64_t tail_pages;   // null: no row has a tail
+  const int32_t* tail_ids; const int32_t* seqused_tail;
+  const int32_t* chunk_start;                                     // [rows + 1]
+  const uint16_t* key; const uint16_t* value;                     // [tokens][heads_kv][128]
+  int64_t key_stride, value_stride;                               // elements per token
+  const uint16_t* key_shift;                                      // nullable [heads_kv][128]
+  int rows, tokens, max_chunk, heads_kv;
+  uint32_t* status;
+};
+
+struct ChunkAttention {
+  ChunkCache c;
+  const uint16_t* query; int64_t q_token_stride, q_head_stride;
+  uint16_t* out; int64_t out_token_stride;
+  float* lse;                                                     // nullable [tokens][heads_q]
+  float* o_partial; float* lse_partial;                           // num_splits > 1: [S][tokens][heads_q][128], [S][tokens][heads_q]
+  int heads_q, num_splits;
+  float scale_log2;                                               // softmax_scale * log2(e)
+};
+
+cudaError_t launch_chunk_attention(const ChunkAttention& a, cudaStream_t stream);
+cudaError_t launch_append_chunk(const ChunkCache& c, int32_t* seqused_fp4_out, int32_t* seqused_tail_out,
+                                cudaStream_t stream);
+cudaError_t launch_dequantize_pages(const ChunkCache& c, const int32_t* page_ids, int count, void* key_out,
+                                    void* value_out, cudaStream_t stream);
+
+// Page pool: reference counts, forks, compaction.
+struct PoolFork {
+  const int32_t* sources; const int32_t* targets; int count;
+  int32_t* page_table; int64_t page_table_stride; int columns, rows;
+  int32_t* pages_held; int32_t* seqused_fp4; int32_t* seqused_tail; const int32_t* row_to_slot;
+  int32_t* refs; int64_t num_pages;
+  uint16_t* tail_key; uint16_t* tail_value; int64_t layer_stride, slot_stride; int layers, slots, heads_kv;
+  uint32_t* status;
+};
+cudaError_t launch_pool_fork(const PoolFork& f, cudaStream_t stream);
+cudaError_t launch_pool_release(const int32_t* list, int count, const int32_t* page_table, int64_t page_table_stride,
+                                int columns, int rows, int32_t* pages_held, int32_t* refs, int64_t num_pages,
+                                uint32_t* status, cudaStream_t stream);
+cudaError_t launch_pool_free_list(const int32_t* refs, int64_t num_pages, int reserved, int32_t* ids, int32_t* count,
+                                  cudaStream_t stream);
+cudaError_t launch_pool_copy(const int64_t* bases, int layers, int64_t pitch, int64_t num_pages, const int32_t* src,
+                             const int32_t* dst, int count, uint32_t* status, cudaStream_t stream);
+cudaError_t launch_pool_compact(const int64_t* bases, int layers, int64_t pitch, int64_t num_pages, int reserved,
+                                int32_t* refs, int32_t* page_table, int64_t page_table_stride, int columns, int rows,
+                                const int32_t* pages_held, int32_t* workspace, int32_t* live_count, uint32_t* status,
+                                cudaStream_t stream);
+
 }  // namespace nvfp4
