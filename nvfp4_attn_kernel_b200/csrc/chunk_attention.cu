@@ -1,75 +1,783 @@
-// Attention of a chunk of new tokens over the paged cache and over the chunk itself (causal).
+// Attention of a chunk of new tokens over the paged cache and, causally, over the chunk itself.
+//
+// Token i of a row sees h history tokens (sealed NVFP4 pages, then the BF16 tail) and the chunk's
+// tokens 0..i.  The G query heads of a KV head and the tokens of a chunk are packed into tiles of
+// 128 query rows, so a K/V tile that has been read (and dequantised) once serves all of them.  A CTA
+// takes one KV head of one row and two streams of work, S = Q K^T and O += P V on the tensor cores
+// (tcgen05, kind::f16, fp32 accumulators in tensor memory), a softmax warpgroup each:
+//   - two tiles of query rows over the same K/V tiles, when the chunk has more than one, or
+//   - one tile of query rows whose K/V tiles the streams take in turns, joined at the end.
+// While one stream computes its softmax the tensor cores work for the other.
+//
+// Operands.  A page's e2m1 * e4m3 is exact in FP16 (six significant bits, 2^-10 to 2688), and FP16
+// probabilities carry eleven bits, so pages meet an FP16 query: rounding a BF16 query row to FP16 loses
+// nothing once its largest magnitude is scaled to [1, 2) by a power of two (what falls below 2^-14 of it is
+// under the fp32 accumulator's own rounding).  Tail and chunk are BF16 as they lie in memory and
+// meet the BF16 query and BF16 probabilities.  The BF16 tiles come first; then each query tile is
+// converted in place, once.
+//
+// Softmax.  A thread owns a query row: running maximum and sum in fp32, exponentials of the scaled
+// scores relative to a maximum that is only replaced when a new one exceeds it by 2^8 (O and the sum are
+// rescaled then; probabilities up to 2^8 fit both formats with the same relative precision).
+#include <cuda_fp16.h>
+
 #include "chunk_common.cuh"
+#include "sm100_device.cuh"
 
 namespace nvfp4 {
 
 namespace {
 
-// One warp per (token, query head); a lane holds four channels.
-__global__ void __launch_bounds__(128)
-chunk_attention_kernel(const ChunkAttention a) {
-  const ChunkCache& c = a.c;
-  const int row = blockIdx.z, head = blockIdx.y, lane = threadIdx.x & 31;
-  const ChunkRow r = resolve_chunk_row(c, row, blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0);
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (i >= r.n) return;
-  const int kvh = head / (a.heads_q / c.heads_kv);
-  const uint16_t* qp = a.query + (int64_t)(r.first + i) * a.q_token_stride + (int64_t)head * a.q_head_stride + lane * 4;
-  float q[4], o[4] = {0, 0, 0, 0};
-  for (int j = 0; j < 4; ++j) q[j] = bf16_bits_to_f32(qp[j]) * a.scale_log2;
-  float m = -INFINITY, l = 0.f;
-  auto fold = [&](const float (&k)[4], const float (&v)[4]) {
-    const float s = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
-    const float top = fmaxf(m, s);
-    const float keep = exp2f(m - top), p = exp2f(s - top);
-    for (int j = 0; j < 4; ++j) o[j] = o[j] * keep + p * v[j];
-    l = l * keep + p;
-    m = top;
-  };
-  for (int pg = 0; pg < r.pages; ++pg) {
-    const int64_t page = c.page_table[(int64_t)row * c.page_table_row_stride + pg];
-    if (page < 0 || page >= c.num_pages) {
-      if (lane == 0) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
-      continue;
+using namespace sm100;
+
+constexpr int kThreads = 512;         // two softmax warpgroups, the producers, the issuer's warpgroup
+constexpr int kProducerWarp0 = 8;
+constexpr int kIssueWarp = 12;
+constexpr int kOperandBytes = 128 * 256;       // 128 rows of 128 16-bit elements: two 128-byte swizzled halves
+constexpr int kHalfBytes = 128 * 128;
+constexpr int kRawBytes = 8192 + 1024;         // a page's nibbles and scales for one head
+constexpr float kRescaleLog2 = 8.f;
+constexpr uint32_t kColS = 0, kColO = 256;     // tensor-memory columns of stream 0; stream 1: + 128
+constexpr float kLn2 = 0.6931471805599453f;
+
+// QTILES query tiles in shared memory, RAW slots of page bytes in flight
+template <int QTILES, int RAW>
+struct ChunkSmem {
+  static constexpr int kQTiles = QTILES, kRaw = RAW;
+  uint8_t q[QTILES][kOperandBytes];
+  uint8_t k[2][kOperandBytes];
+  uint8_t v[2][kOperandBytes];
+  uint8_t raw[RAW][kRawBytes];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_ready[2], o_done[2], q_f16[2], all_done;
+  float join[2][128];        // stream 1's maximum and sum, when the streams share a tile
+  int tile_valid[8];         // K/V positions of tile t that exist (0: a refused page), at t % 8: the producers are at
+                             // most three tiles ahead of the operands, the softmax at most two behind them
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+__device__ __forceinline__ uint32_t swizzled(int row, int unit) {   // 16-byte unit 0..15 of a row
+  return (uint32_t)((unit >> 3) * kHalfBytes + row * 128 + (((unit ^ row) & 7) << 4));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const uint32_t bytes = valid ? 16 : 0;     // 0: the destination is zero-filled
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp_async_wait_most(int pending) {   // at most `pending` groups left in flight
+  switch (pending) {
+    case 0: cp_async_wait<0>(); break;
+    case 1: cp_async_wait<1>(); break;
+    case 2: cp_async_wait<2>(); break;
+    case 3: cp_async_wait<3>(); break;
+    case 4: cp_async_wait<4>(); break;
+    case 5: cp_async_wait<5>(); break;
+    default: cp_async_wait<6>(); break;
+  }
+}
+
+// Descriptors of a 16-bit operand tile, 128-byte swizzle, eight-row groups 1024 bytes apart.  K-major:
+// a row's 64 elements are contiguous (the leading offset is not used).  MN-major (V of BF16 tiles, rows
+// are tokens): the leading offset leads to the next 64 channels.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(kHalfBytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// M = 128, N = 128, fp32 accumulators; A and B both FP16 (0) or both BF16 (1)
+__device__ __forceinline__ uint32_t idesc(bool bf16, bool b_mn_major) {
+  const uint32_t f = bf16 ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
+      : "memory");
+}
+
+#define NVFP4_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define NVFP4_W8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+
+// 32 columns of this warp's 32 lanes; the caller waits (tmem_ld_wait)
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : NVFP4_R8(r, 0), NVFP4_R8(r, 8), NVFP4_R8(r, 16), NVFP4_R8(r, 24)
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      NVFP4_W8(r, 0), NVFP4_W8(r, 8), NVFP4_W8(r, 16), NVFP4_W8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Four bytes of nibbles -> four FP16 pairs (nibble 2i in the low half of pair i).
+__device__ __forceinline__ void e2m1x8_to_f16x8(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+  return h;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// What a CTA works on.
+struct Work {
+  ChunkRow r;
+  int group, tile_tokens;      // query heads per KV head; tokens in a tile of query rows
+  int token0;                  // first chunk token of tile 0
+  bool two;                    // two tiles of query rows; else one, the streams taking turns
+  int fresh, tail_tiles;       // K/V tiles: the chunk's, then the tail's (0 or 1), then the pages
+  int begin, end;              // this split's range of them
+  int bf16_tiles;              // of these, how many are BF16
+  int steps;                   // softmax steps of both streams together
+};
+
+__device__ __forceinline__ int stream_steps(const Work& w, int stream) {
+  return w.two ? w.end - w.begin : (w.end - w.begin + 1 - stream) >> 1;
+}
+
+// The biased exponent e of a query row's largest magnitude (BF16 bits without sign): the row times 2^(127 - e)
+// lies within [1, 2).  Both powers of two are normal numbers: e from 1 (zero and subnormal rows) to 253 (the two
+// largest binades end below 4 instead); rows that are not finite stay as they are.
+__device__ __forceinline__ int row_exponent(uint32_t amax_bits) {
+  const int e = amax_bits >> 7;
+  return e == 255 ? 127 : min(max(e, 1), 253);
+}
+__device__ __forceinline__ float exponent_value(int biased) { return __uint_as_float((uint32_t)biased << 23); }
+__device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t w, float factor) {
+  const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * factor, __uint_as_float(w & 0xFFFF0000u) * factor);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 bf16x8_to_f16x8(const uint4& v, float f) {
+  return make_uint4(bf16x2_to_f16x2(v.x, f), bf16x2_to_f16x2(v.y, f), bf16x2_to_f16x2(v.z, f), bf16x2_to_f16x2(v.w, f));
+}
+
+// -- producers -----------------------------------------------------------------------------------
+
+// Items of K/V work in order: 2 t = K of tile t, 2 t + 1 = V of tile t (t from the split's first tile).
+template <class SM>
+struct Producer {
+  const ChunkAttention& a;
+  SM& sm;
+  const Work& w;
+  int row, kvh, warp, lane;
+  int page_base = -1;       // first of the 32 page-table entries that the lanes hold
+  int page_mine = 0;
+
+  __device__ __forceinline__ int64_t page_of(int p) {
+    if (page_base < 0 || p >= page_base + 32) {
+      page_base = p;
+      const int at = p + lane;
+      page_mine = at < w.r.pages ? a.c.page_table[(int64_t)row * a.c.page_table_row_stride + at] : -1;
     }
-    const uint8_t* ks = c.k_sf + page * c.k_sf_pitch + kvh * kSfBlockBytes;
-    const uint8_t* vs = c.v_sf + page * c.v_sf_pitch + kvh * kSfBlockBytes;
-    for (int t = 0; t < kPage; ++t) {
-      const uint16_t n = *reinterpret_cast<const uint16_t*>(c.k_packed + page * c.k_pitch +
-                                                            ((int64_t)t * c.heads_kv + kvh) * 64 + lane * 2);
-      const float s = e4m3_to_f32(ks[sf_offset(t, lane >> 2)]);
-      float k[4], v[4];
+    return __shfl_sync(0xffffffffu, page_mine, p - page_base);
+  }
+
+  // 128 tokens of BF16 rows straight into an operand tile
+  __device__ __forceinline__ void issue_bf16(int tile, bool is_v, uint32_t dst) {
+    const ChunkCache& c = a.c;
+    const uint16_t* src;
+    int64_t stride;
+    int valid;
+    if (tile < w.fresh) {
+      stride = is_v ? c.value_stride : c.key_stride;
+      src = (is_v ? c.value : c.key) + ((int64_t)w.r.first + tile * 128) * stride + kvh * kHeadDim;
+      valid = min(128, w.r.n - tile * 128);
+    } else {
+      stride = (int64_t)c.heads_kv * kHeadDim;
+      src = (is_v ? c.tail_value : c.tail_key) + (int64_t)w.r.tail_id * kPage * stride + kvh * kHeadDim;
+      valid = w.r.tail;
+    }
+    const int unit = lane & 15;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const int tok = warp * 32 + i * 2 + (lane >> 4);
+      const bool ok = tok < valid;
+      cp_async16(dst + swizzled(tok, unit), src + (ok ? tok : 0) * stride + unit * 8, ok);
+    }
+    if (!is_v && warp == 0 && lane == 0) sm.tile_valid[(tile - w.begin) & 7] = valid;
+  }
+
+  // this warp's 32 rows of a page's nibbles and scales into a raw slot
+  __device__ __forceinline__ void issue_page(int tile, bool is_v, uint8_t* slot) {
+    const ChunkCache& c = a.c;
+    const int64_t page = page_of(tile - w.fresh - w.tail_tiles);
+    const bool ok = page >= 0 && page < c.num_pages;
+    if (!is_v && warp == 0 && lane == 0) {
+      sm.tile_valid[(tile - w.begin) & 7] = ok ? 128 : 0;
+      if (!ok) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
+    }
+    const int64_t at = ok ? page : 0;
+    const uint8_t* packed = is_v ? c.v_packed + at * c.v_pitch + (int64_t)kvh * 8192 : c.k_packed + at * c.k_pitch + kvh * 64;
+    const uint8_t* scales = (is_v ? c.v_sf + at * c.v_sf_pitch : c.k_sf + at * c.k_sf_pitch) + kvh * kSfBlockBytes;
+    const int64_t stride = is_v ? 64 : (int64_t)c.heads_kv * 64;
+    const uint32_t dst = smem_u32(slot);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = warp * 32 + i * 8 + (lane >> 2), piece = lane & 3;
+      cp_async16(dst + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4), packed + r * stride + piece * 16, ok);
+    }
+    if (ok) {
+      cp_async4(dst + 8192 + warp * 256 + lane * 8, scales + lane * 16 + warp * 4);
+      cp_async4(dst + 8192 + warp * 256 + lane * 8 + 4, scales + 512 + lane * 16 + warp * 4);
+    } else {      // a refused page: zeros everywhere, its scores are masked
+      *reinterpret_cast<uint2*>(slot + 8192 + warp * 256 + lane * 8) = make_uint2(0, 0);
+    }
+  }
+
+  // row warp * 32 + lane of a raw slot, dequantised into an operand tile
+  __device__ __forceinline__ void expand(const uint8_t* slot, uint8_t* dst) {
+    const int r = warp * 32 + lane;
+    const uint2 s = *reinterpret_cast<const uint2*>(slot + 8192 + warp * 256 + lane * 8);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const uint4 n = *reinterpret_cast<const uint4*>(slot + r * 64 + ((p ^ ((r >> 1) & 3)) << 4));
+      const uint32_t two = e4m3x2_to_f16x2(((p & 2) ? s.y : s.x) >> ((p & 1) * 16));
+      const uint32_t s0 = __byte_perm(two, two, 0x1010), s1 = __byte_perm(two, two, 0x3232);
+      const uint32_t words[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
       for (int j = 0; j < 4; ++j) {
-        k[j] = e2m1_to_f32(n >> (4 * j)) * s;
-        const int ch = lane * 4 + j;
-        const uint8_t b = c.v_packed[page * c.v_pitch + ((int64_t)kvh * kHeadDim + ch) * 64 + t / 2];
-        v[j] = e2m1_to_f32(b >> (4 * (t & 1))) * e4m3_to_f32(vs[sf_offset(ch, t >> 4)]);
+        uint32_t h[4];
+        e2m1x8_to_f16x8(words[j], h);
+        const uint32_t sc = j < 2 ? s0 : s1;
+        *reinterpret_cast<uint4*>(dst + swizzled(r, p * 4 + j)) =
+            make_uint4(hmul2(h[0], sc), hmul2(h[1], sc), hmul2(h[2], sc), hmul2(h[3], sc));
       }
-      fold(k, v);
     }
   }
-  for (int t = 0; t < r.tail + i + 1; ++t) {
-    const bool old = t < r.tail;
-    const int64_t tok = old ? (int64_t)r.tail_id * kPage + t : (int64_t)r.first + t - r.tail;
-    const uint16_t* kp = old ? c.tail_key + (tok * c.heads_kv + kvh) * kHeadDim : c.key + tok * c.key_stride + kvh * kHeadDim;
-    const uint16_t* vp = old ? c.tail_value + (tok * c.heads_kv + kvh) * kHeadDim : c.value + tok * c.value_stride + kvh * kHeadDim;
-    float k[4], v[4];
-    for (int j = 0; j < 4; ++j) {
-      k[j] = bf16_bits_to_f32(kp[lane * 4 + j]);
-      if (!old && c.key_shift) k[j] -= bf16_bits_to_f32(c.key_shift[kvh * kHeadDim + lane * 4 + j]);
-      v[j] = bf16_bits_to_f32(vp[lane * 4 + j]);
+};
+
+template <class SM>
+__device__ __forceinline__ void produce(const ChunkAttention& a, SM& sm, const Work& w, int row, int kvh, int warp, int lane) {
+  constexpr int RAW = SM::kRaw;
+  Producer<SM> p{a, sm, w, row, kvh, warp, lane};
+  const int items = 2 * (w.end - w.begin), first_page_item = 2 * w.bf16_tiles;
+  int issued = 0;
+  for (int item = 0; item < items; ++item) {
+    // Issue ahead: BF16 items go straight into an operand stage, two items (the next tile's same operand) ahead,
+    // once that stage is empty; a third would wait for products that wait for this item.  Page items go into the
+    // raw slot that the item RAW before them has left.
+    while (issued < items && (issued < first_page_item ? issued <= item + 2 : issued < item + RAW)) {
+      const int t = issued >> 1;
+      const bool is_v = issued & 1;
+      if (issued < first_page_item) {
+        if (t >= 2 && !mbar_wait(is_v ? &sm.v_empty[t & 1] : &sm.k_empty[t & 1], ((t >> 1) - 1) & 1, sm, a.c.status)) goto out;
+        p.issue_bf16(w.begin + t, is_v, smem_u32(is_v ? sm.v[t & 1] : sm.k[t & 1]));
+      } else {
+        p.issue_page(w.begin + t, is_v, sm.raw[issued % RAW]);
+      }
+      cp_async_commit();
+      ++issued;
     }
-    fold(k, v);
+    cp_async_wait_most(issued - item - 1);
+    __syncwarp();
+    {
+      const int t = item >> 1;
+      const bool is_v = item & 1;
+      if (item >= first_page_item) {
+        if (t >= 2 && !mbar_wait(is_v ? &sm.v_empty[t & 1] : &sm.k_empty[t & 1], ((t >> 1) - 1) & 1, sm, a.c.status)) goto out;
+        p.expand(sm.raw[item % RAW], is_v ? sm.v[t & 1] : sm.k[t & 1]);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(is_v ? &sm.v_full[t & 1] : &sm.k_full[t & 1]);
+    }
   }
-  uint16_t* out = a.out + (int64_t)(r.first + i) * a.out_token_stride + head * kHeadDim + lane * 4;
-  for (int j = 0; j < 4; ++j) out[j] = __bfloat16_as_ushort(__float2bfloat16_rn(o[j] / l));
-  if (a.lse && lane == 0) a.lse[(int64_t)(r.first + i) * a.heads_q + head] = (m + log2f(l)) * 0.6931471805599453f;
+out:
+  cp_async_wait<0>();
+}
+
+// -- issuer --------------------------------------------------------------------------------------
+
+template <class SM>
+__device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem) {
+  uint32_t* status = a.c.status;
+  bool ok = true;
+  bool f16_seen[2] = {w.bf16_tiles == 0, w.bf16_tiles == 0};
+  auto scores = [&](int step) {
+    const int s = step & 1, t = w.two ? step >> 1 : step, qt = w.two ? s : 0;
+    const bool bf16 = t < w.bf16_tiles;
+    ok = ok && mbar_wait(&sm.k_full[t & 1], (t >> 1) & 1, sm, status);
+    if (!bf16 && !f16_seen[qt]) {
+      ok = ok && mbar_wait(&sm.q_f16[qt], 0, sm, status);
+      f16_seen[qt] = true;
+    }
+    if (!ok) return;
+    tc_fence_after();
+    const uint32_t q = smem_u32(sm.q[SM::kQTiles > 1 ? qt : 0]), k = smem_u32(sm.k[t & 1]);
+    const uint32_t id = idesc(bf16, false);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t at = (i >> 2) * kHalfBytes + (i & 3) * 32;
+      mma_ss(tmem + kColS + s * 128, desc_k_major(q + at), desc_k_major(k + at), id, i > 0);
+    }
+    mma_commit(&sm.s_full[s]);
+    if (!w.two || s == 1) mma_commit(&sm.k_empty[t & 1]);
+  };
+  scores(0);
+  if (w.steps > 1) scores(1);
+  for (int step = 0; step < w.steps && ok; ++step) {
+    const int s = step & 1, t = w.two ? step >> 1 : step, u = step >> 1;
+    const bool bf16 = t < w.bf16_tiles;
+    ok = ok && mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, sm, status);
+    ok = ok && mbar_wait(&sm.p_ready[s], u & 1, sm, status);
+    if (!ok) break;
+    tc_fence_after();
+    const uint32_t v = smem_u32(sm.v[t & 1]);
+    const uint32_t id = idesc(bf16, bf16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t b = bf16 ? desc_mn_major(v + i * 2048) : desc_k_major(v + (i >> 2) * kHalfBytes + (i & 3) * 32);
+      mma_ts(tmem + kColO + s * 128, tmem + kColS + s * 128 + i * 8, b, id, u > 0 || i > 0);
+    }
+    mma_commit(&sm.o_done[s]);
+    if (!w.two || s == 1) mma_commit(&sm.v_empty[t & 1]);
+    if (step + 2 < w.steps) scores(step + 2);
+  }
+  mma_commit(&sm.all_done);
+}
+
+// -- softmax -------------------------------------------------------------------------------------
+
+// A thread's query row.
+struct QueryRow {
+  int token, head;       // of the chunk; query head
+  bool live;
+  int exponent;          // see row_exponent
+  float shift;           // q . key_shift
+};
+
+__device__ __forceinline__ QueryRow query_row(const ChunkAttention& a, const Work& w, int kvh, int tile, int r) {
+  QueryRow q;
+  const int in_tile = r / w.group;
+  q.token = w.token0 + tile * w.tile_tokens + in_tile;
+  q.head = kvh * w.group + r - in_tile * w.group;
+  q.live = in_tile < w.tile_tokens && q.token < w.r.n;
+  q.exponent = 127;
+  q.shift = 0.f;
+  return q;
+}
+
+// Reads the row, finds its exponent and its product with the key shift, and (store) lays it out as an operand:
+// BF16, or FP16 at once when no K/V tile of the split is BF16.
+__device__ __forceinline__ void load_query(const ChunkAttention& a, const Work& w, int kvh, int r, QueryRow& q, uint8_t* dst,
+                                           bool store) {
+  uint4 x[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = make_uint4(0, 0, 0, 0);
+  if (q.live) {
+    const uint16_t* src = a.query + (int64_t)(w.r.first + q.token) * a.q_token_stride + (int64_t)q.head * a.q_head_stride;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * 8);
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu),
+                                 __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
+  }
+  q.exponent = row_exponent(max(top & 0xFFFFu, top >> 16));
+  if (a.c.key_shift && w.fresh > w.begin) {
+    const uint16_t* mu = a.c.key_shift + kvh * kHeadDim;
+    float even = 0.f, odd = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint4 y = *reinterpret_cast<const uint4*>(mu + i * 8);
+      float u[8], v[8];
+      unpack_bf16x8(x[i], u);
+      unpack_bf16x8(y, v);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        even += u[j] * v[j];
+        odd += u[j + 1] * v[j + 1];
+      }
+    }
+    q.shift = even + odd;
+  }
+  if (!store) return;
+  const float f = exponent_value(254 - q.exponent);
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    *reinterpret_cast<uint4*>(dst + swizzled(r, i)) = w.bf16_tiles ? x[i] : bf16x8_to_f16x8(x[i], f);
+}
+
+__device__ __forceinline__ void query_to_f16(uint8_t* tile, int r, int exponent) {
+  const float f = exponent_value(254 - exponent);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    uint4* at = reinterpret_cast<uint4*>(tile + swizzled(r, i));
+    *at = bf16x8_to_f16x8(*at, f);
+  }
+}
+
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
+  uint32_t b, h;
+  if (bf16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(hi), "f"(lo));
+    return b;
+  }
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
+  return h;
+}
+
+struct RowState { float m, l; };    // maximum in use (log2 units) and the sum relative to it
+
+template <class SM>
+__device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int stream, int r,
+                                        const QueryRow& q, RowState& state) {
+  uint32_t* status = a.c.status;
+  constexpr uint32_t kAll = 0xffffffffu;
+  const int qt = w.two ? stream : 0;
+  const uint32_t lanes = (uint32_t)(r & ~31) << 16;
+  const uint32_t col_s = tmem + lanes + kColS + stream * 128, col_o = tmem + lanes + kColO + stream * 128;
+  const bool warp_live = __any_sync(kAll, q.live);
+  // a score in log2 units: against the BF16 query, and against the row's FP16 form (never zero, so that a masked
+  // -inf stays -inf)
+  const float scale_bf16 = a.scale_log2;
+  const float scale_f16 = fmaxf(a.scale_log2 * exponent_value(q.exponent), 1.2e-38f);
+  float m = -INFINITY, l = 0.f;
+  const int steps = stream_steps(w, stream);
+  for (int u = 0; u < steps; ++u) {
+    const int t = w.two ? u : 2 * u + stream, tile = w.begin + t;
+    if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream], u & 1, sm, status))) return false;
+    tc_fence_after();
+    const bool bf16 = t < w.bf16_tiles;
+    if (t == w.bf16_tiles - 1 && w.bf16_tiles < w.end - w.begin) {
+      // every product with the BF16 query that this tile is in has been formed: its rows become FP16
+      query_to_f16(sm.q[SM::kQTiles > 1 ? qt : 0], r, q.exponent);
+      fence_proxy_async();
+      mbar_arrive(&sm.q_f16[qt]);
+    }
+    if (warp_live) {
+      uint32_t raw[128];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld32(col_s + i * 32, raw + i * 32);
+      tmem_ld_wait();
+      const float scale = bf16 ? scale_bf16 : scale_f16;
+      const float offset = tile < w.fresh ? q.shift * scale : 0.f;
+      const int limit = tile < w.fresh ? q.token - tile * 128 + 1 : sm.tile_valid[t & 7];
+      if (__any_sync(kAll, limit < 128)) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 128; i += 8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          top[j] = fmaxf(fmaxf(top[j], __uint_as_float(raw[i + 2 * j])), __uint_as_float(raw[i + 2 * j + 1]));
+      }
+      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const float now = best == -INFINITY ? -INFINITY : best * scale - offset;
+      const bool grows = now > m + kRescaleLog2;
+      if (__any_sync(kAll, grows)) {
+        const float alpha = grows ? ex2(m - now) : 1.f;       // 0 from an empty row
+        if (u > 0) {
+          if (!__all_sync(kAll, mbar_wait(&sm.o_done[stream], (u - 1) & 1, sm, status))) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o[32];
+            tmem_ld32(col_o + i * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tmem_st32(col_o + i * 32, o);
+          }
+        }
+        l *= alpha;
+        if (grows) m = now;
+      }
+      const float base = (m == -INFINITY ? 0.f : m) + offset;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int c = half * 64 + 2 * i;
+          const float x = ex2(fmaf(__uint_as_float(raw[c]), scale, -base));
+          const float y = ex2(fmaf(__uint_as_float(raw[c + 1]), scale, -base));
+          sum[(2 * i) & 3] += x;
+          sum[(2 * i + 1) & 3] += y;
+          p[i] = pack16(x, y, bf16);
+        }
+        tmem_st32(col_s + half * 32, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+    }
+    tc_fence_before();
+    mbar_arrive(&sm.p_ready[stream]);
+  }
+  state.m = m;
+  state.l = l;
+  return true;
+}
+
+// Rows out: divided by the sum, as BF16, or as a normalised fp32 partial with its log2-sum.
+template <class SM>
+__device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int stream, int r,
+                                       const QueryRow& q, const RowState& state, int split, bool ok) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  const bool join = !w.two && w.steps > 1;      // stream 1 has a part of the same rows
+  ok = __all_sync(kAll, ok && mbar_wait(&sm.all_done, 0, sm, a.c.status));
+  tc_fence_after();
+  const uint32_t lanes = (uint32_t)(r & ~31) << 16;
+  const uint32_t col_o = tmem + lanes + kColO + stream * 128;
+  float* shared_o = reinterpret_cast<float*>(sm.k);     // [channel][row]: every product has been formed
+  if (join) {
+    if (stream == 1) {
+      if (ok) {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          uint32_t o[32];
+          tmem_ld32(col_o + i * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) shared_o[(i * 32 + j) * 128 + r] = __uint_as_float(o[j]);
+        }
+      }
+      sm.join[0][r] = state.m;
+      sm.join[1][r] = state.l;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+  }
+  if (!ok || sm.abort_flag || (!w.two && stream == 1)) return;
+  float w0 = 1.f, w1 = 0.f, m = state.m, l = state.l;
+  if (join) {
+    const float m1 = sm.join[0][r];
+    m = fmaxf(state.m, m1);
+    w0 = state.m == -INFINITY ? 0.f : ex2(state.m - m);
+    w1 = m1 == -INFINITY ? 0.f : ex2(m1 - m);
+    l = state.l * w0 + sm.join[1][r] * w1;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  w0 *= inv;
+  w1 *= inv;
+  const int64_t token = (int64_t)w.r.first + q.token;
+  const bool partial = a.num_splits > 1;
+  const int64_t part = ((int64_t)split * a.c.tokens + token) * a.heads_q + q.head;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    uint32_t o[32];
+    __syncwarp();
+    tmem_ld32(col_o + i * 32, o);
+    tmem_ld_wait();
+    float x[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(o[j]) * w0;
+    if (join) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] += shared_o[(i * 32 + j) * 128 + r] * w1;
+    }
+    if (q.live && partial) {
+      float4* dst = reinterpret_cast<float4*>(a.o_partial + part * kHeadDim + i * 32);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dst[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+    } else if (q.live) {
+      uint4* dst = reinterpret_cast<uint4*>(a.out + token * a.out_token_stride + q.head * kHeadDim + i * 32);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        dst[j] = make_uint4(pack16(x[8 * j], x[8 * j + 1], true), pack16(x[8 * j + 2], x[8 * j + 3], true),
+                            pack16(x[8 * j + 4], x[8 * j + 5], true), pack16(x[8 * j + 6], x[8 * j + 7], true));
+    }
+  }
+  if (q.live) {
+    const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+    if (partial) a.lse_partial[part] = lse2;
+    else if (a.lse) a.lse[token * a.heads_q + q.head] = lse2 * kLn2;
+  }
+}
+
+// grid (query blocks * splits, heads_kv, rows)
+template <int QTILES, int RAW>
+__global__ void __launch_bounds__(kThreads, 1)
+chunk_attention_kernel(const ChunkAttention a, int query_blocks) {
+  using SM = ChunkSmem<QTILES, RAW>;
+  extern __shared__ uint8_t smem_raw[];
+  SM& sm = *reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int row = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the blocks with the longest causal reach first
+  const int split = blockIdx.x / query_blocks, block = query_blocks - 1 - (blockIdx.x - split * query_blocks);
+  Work w;
+  w.r = resolve_chunk_row(a.c, row, blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0);
+  w.group = a.heads_q / a.c.heads_kv;
+  w.tile_tokens = 128 / w.group;
+  w.token0 = block * QTILES * w.tile_tokens;
+  if (w.token0 >= w.r.n) return;
+  w.two = QTILES > 1 && w.token0 + w.tile_tokens < w.r.n;
+  const int last_token = min(w.r.n, w.token0 + (w.two ? 2 : 1) * w.tile_tokens);
+  w.fresh = (last_token + 127) >> 7;
+  w.tail_tiles = w.r.tail > 0;
+  const int tiles = w.fresh + w.tail_tiles + w.r.pages;
+  const int per = (tiles + a.num_splits - 1) / a.num_splits;
+  w.begin = min(split * per, tiles);
+  w.end = min(w.begin + per, tiles);
+  w.bf16_tiles = max(0, min(w.end, w.fresh + w.tail_tiles) - w.begin);
+  w.steps = (w.two ? 2 : 1) * (w.end - w.begin);
+  const int stream = warp >> 2, r = threadIdx.x & 127;
+  if (w.begin == w.end) {      // nothing in this range of the keys
+    if (stream < (w.two ? 2 : 1)) {
+      const QueryRow q = query_row(a, w, kvh, stream, r);
+      if (q.live) a.lse_partial[((int64_t)split * a.c.tokens + w.r.first + q.token) * a.heads_q + q.head] = -INFINITY;
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.k_full[i], 4);
+      mbar_init(&sm.v_full[i], 4);
+      mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_ready[i], 128);
+      mbar_init(&sm.o_done[i], 1);
+      mbar_init(&sm.q_f16[i], 128);
+    }
+    mbar_init(&sm.all_done, 1);
+    sm.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kIssueWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem_base))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  QueryRow q{};
+  if (stream < 2) {
+    const int tile = w.two ? stream : 0;
+    q = query_row(a, w, kvh, tile, r);
+    load_query(a, w, kvh, r, q, sm.q[QTILES > 1 ? tile : 0], w.two || stream == 0);
+    fence_proxy_async();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  // registers: 512 threads at 128, shared out as 2 x 192 + 88 + 40 = 4 x 128
+  if (stream < 2) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    RowState state{-INFINITY, 0.f};
+    const bool ok = softmax(a, sm, w, tmem, stream, r, q, state);
+    finish(a, sm, w, tmem, stream, r, q, state, split, ok);
+  } else if (stream == 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    produce(a, sm, w, row, kvh, warp - kProducerWarp0, lane);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == kIssueWarp) {
+      if (lane == 0) {
+        issue(a, sm, w, tmem);
+        // nothing of this CTA's is in flight when its tensor memory goes back, also after an expired wait
+        const unsigned long long t0 = global_ns();
+        while (!mbar_try(&sm.all_done, 0) && global_ns() - t0 < 200000000ull) {}
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssueWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// Joins the splits of a row's tokens: one warp per (token, query head), a lane holds four channels.
+constexpr int kMergeWarps = 8;
+__global__ void __launch_bounds__(32 * kMergeWarps)
+chunk_merge_kernel(const ChunkAttention a) {
+  const int lane = threadIdx.x & 31;
+  const ChunkRow r = resolve_chunk_row(a.c, blockIdx.y, false);
+  const int64_t unit = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  const int i = (int)(unit / a.heads_q), head = (int)(unit - (int64_t)i * a.heads_q);
+  if (i >= r.n) return;
+  const int64_t token = (int64_t)r.first + i;
+  const int64_t at = token * a.heads_q + head, pitch = (int64_t)a.c.tokens * a.heads_q;
+  float top = -INFINITY;
+  for (int s = lane; s < a.num_splits; s += 32) top = fmaxf(top, a.lse_partial[s * pitch + at]);
+  top = warp_max(top);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.f;
+  for (int s = 0; s < a.num_splits; ++s) {
+    const float lse = a.lse_partial[s * pitch + at];
+    if (lse == -INFINITY) continue;           // an empty range wrote no rows
+    const float4 x = *reinterpret_cast<const float4*>(a.o_partial + (s * pitch + at) * kHeadDim + lane * 4);
+    const float weight = ex2(lse - top);
+    total += weight;
+    o.x += weight * x.x; o.y += weight * x.y; o.z += weight * x.z; o.w += weight * x.w;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  *reinterpret_cast<uint2*>(a.out + token * a.out_token_stride + head * kHeadDim + lane * 4) =
+      make_uint2(pack16(o.x * inv, o.y * inv, true), pack16(o.z * inv, o.w * inv, true));
+  if (a.lse && lane == 0) a.lse[at] = (top + log2f(total)) * kLn2;
+}
+
+template <int QTILES, int RAW>
+cudaError_t launch(const ChunkAttention& a, cudaStream_t stream) {
+  const int bytes = (int)sizeof(ChunkSmem<QTILES, RAW>) + 1024;
+  static_assert(sizeof(ChunkSmem<QTILES, RAW>) + 1024 <= 232448, "shared memory of one CTA");
+  cudaError_t e = cudaFuncSetAttribute(chunk_attention_kernel<QTILES, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  const int tokens = 128 / (a.heads_q / a.c.heads_kv) * QTILES;
+  const int blocks = (a.c.max_chunk + tokens - 1) / tokens;
+  chunk_attention_kernel<QTILES, RAW><<<dim3(blocks * a.num_splits, a.c.heads_kv, a.c.rows), kThreads, bytes, stream>>>(a, blocks);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_chunk_attention(const ChunkAttention& a, cudaStream_t stream) {
-  chunk_attention_kernel<<<dim3((a.c.max_chunk + 3) / 4, a.heads_q, a.c.rows), 128, 0, stream>>>(a);
+  // one tile of query rows holds 128 / G tokens: longer chunks pair tiles, shorter ones leave the second tile's
+  // shared memory to page bytes in flight
+  const int tile_tokens = 128 / (a.heads_q / a.c.heads_kv);
+  cudaError_t e = a.c.max_chunk > tile_tokens ? launch<2, 3>(a, stream) : launch<1, 7>(a, stream);
+  if (e != cudaSuccess || a.num_splits == 1) return e;
+  const int64_t units = (int64_t)a.c.max_chunk * a.heads_q;
+  chunk_merge_kernel<<<dim3((unsigned)((units + kMergeWarps - 1) / kMergeWarps), a.c.rows), 32 * kMergeWarps, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
