@@ -32,7 +32,7 @@ using namespace sm100;
 
 constexpr int kThreads = 512;         // two softmax warpgroups, the producers, the issuer's warpgroup
 constexpr int kProducerWarp0 = 8;
-constexpr int kIssueWarp = 12;
+constexpr int kIssueWarp = 12;        // and 13: one per stream
 constexpr int kOperandBytes = 128 * 256;       // 128 rows of 128 16-bit elements: two 128-byte swizzled halves
 constexpr int kHalfBytes = 128 * 128;
 constexpr int kRawBytes = 8192 + 1024;         // a page's nibbles and scales for one head
@@ -100,16 +100,30 @@ __device__ __forceinline__ uint32_t idesc(bool bf16, bool b_mn_major) {
   return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+// Issued by the lane whose `leader` is set, out of a warp that runs converged.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+  return leader;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id),
+      "r"(accumulate), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id),
+      "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leader)
       : "memory");
 }
 
@@ -329,54 +343,65 @@ out:
   cp_async_wait<0>();
 }
 
-// -- issuer --------------------------------------------------------------------------------------
+// -- issuers -------------------------------------------------------------------------------------
 
+// One warp per stream: scores of tile t, then, step by step, P V of a tile and the scores of the next one (which
+// overwrite the tensor-memory columns that P sat in; the products of one thread complete in order).  The whole warp
+// runs the loop, so addresses and descriptors stay in uniform registers; one elected lane issues.
 template <class SM>
-__device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem) {
+__device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int s) {
+  constexpr uint32_t kAll = 0xffffffffu;
   uint32_t* status = a.c.status;
-  bool ok = true;
-  bool f16_seen[2] = {w.bf16_tiles == 0, w.bf16_tiles == 0};
-  auto scores = [&](int step) {
-    const int s = step & 1, t = w.two ? step >> 1 : step, qt = w.two ? s : 0;
+  const uint32_t leader = elect_one();
+  const int qt = w.two ? s : 0, first = w.two ? 0 : s, stride = w.two ? 1 : 2;
+  const int tiles = w.end - w.begin;
+  const uint64_t q_desc = desc_k_major(smem_u32(sm.q[SM::kQTiles > 1 ? qt : 0]));
+  const uint32_t col_s = tmem + kColS + s * 128, col_o = tmem + kColO + s * 128;
+  bool f16_seen = w.bf16_tiles == 0;
+  auto scores = [&](int t) -> bool {
     const bool bf16 = t < w.bf16_tiles;
-    ok = ok && mbar_wait(&sm.k_full[t & 1], (t >> 1) & 1, sm, status);
-    if (!bf16 && !f16_seen[qt]) {
+    bool ok = mbar_wait(&sm.k_full[t & 1], (t >> 1) & 1, sm, status);
+    if (!bf16 && !f16_seen) {
       ok = ok && mbar_wait(&sm.q_f16[qt], 0, sm, status);
-      f16_seen[qt] = true;
+      f16_seen = true;
     }
-    if (!ok) return;
+    if (!__all_sync(kAll, ok)) return false;
     tc_fence_after();
-    const uint32_t q = smem_u32(sm.q[SM::kQTiles > 1 ? qt : 0]), k = smem_u32(sm.k[t & 1]);
+    const uint64_t k_desc = desc_k_major(smem_u32(sm.k[t & 1]));
     const uint32_t id = idesc(bf16, false);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t at = (i >> 2) * kHalfBytes + (i & 3) * 32;
-      mma_ss(tmem + kColS + s * 128, desc_k_major(q + at), desc_k_major(k + at), id, i > 0);
+      const uint64_t at = ((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4;
+      mma_ss(col_s, q_desc + at, k_desc + at, id, i > 0, leader);
     }
-    mma_commit(&sm.s_full[s]);
-    if (!w.two || s == 1) mma_commit(&sm.k_empty[t & 1]);
+    commit(&sm.s_full[s], leader);
+    commit(&sm.k_empty[t & 1], leader);
+    return true;
   };
-  scores(0);
-  if (w.steps > 1) scores(1);
-  for (int step = 0; step < w.steps && ok; ++step) {
-    const int s = step & 1, t = w.two ? step >> 1 : step, u = step >> 1;
+  bool ok = first < tiles && scores(first);
+  for (int t = first, u = 0; t < tiles && ok; t += stride, ++u) {
     const bool bf16 = t < w.bf16_tiles;
-    ok = ok && mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, sm, status);
+    ok = mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, sm, status);
     ok = ok && mbar_wait(&sm.p_ready[s], u & 1, sm, status);
-    if (!ok) break;
+    if (!__all_sync(kAll, ok)) break;
     tc_fence_after();
     const uint32_t v = smem_u32(sm.v[t & 1]);
     const uint32_t id = idesc(bf16, bf16);
+    if (bf16) {
+      const uint64_t v_desc = desc_mn_major(v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint64_t b = bf16 ? desc_mn_major(v + i * 2048) : desc_k_major(v + (i >> 2) * kHalfBytes + (i & 3) * 32);
-      mma_ts(tmem + kColO + s * 128, tmem + kColS + s * 128 + i * 8, b, id, u > 0 || i > 0);
+      for (int i = 0; i < 8; ++i) mma_ts(col_o, col_s + i * 8, v_desc + i * (2048 >> 4), id, u > 0 || i > 0, leader);
+    } else {
+      const uint64_t v_desc = desc_k_major(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        mma_ts(col_o, col_s + i * 8, v_desc + (((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4), id, u > 0 || i > 0, leader);
     }
-    mma_commit(&sm.o_done[s]);
-    if (!w.two || s == 1) mma_commit(&sm.v_empty[t & 1]);
-    if (step + 2 < w.steps) scores(step + 2);
+    commit(&sm.o_done[s], leader);
+    commit(&sm.v_empty[t & 1], leader);
+    if (t + stride < tiles) ok = scores(t + stride);
   }
-  mma_commit(&sm.all_done);
+  commit(&sm.all_done, leader);
 }
 
 // -- softmax -------------------------------------------------------------------------------------
@@ -485,7 +510,11 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
     tc_fence_after();
     const bool bf16 = t < w.bf16_tiles;
     if (t == w.bf16_tiles - 1 && w.bf16_tiles < w.end - w.begin) {
-      // every product with the BF16 query that this tile is in has been formed: its rows become FP16
+      // the last product with the BF16 query: once the other stream's is done too where they share it (its next
+      // one waits for what follows), the rows become FP16
+      if (!w.two && t > 0 &&
+          !__all_sync(kAll, mbar_wait(&sm.s_full[stream ^ 1], ((t - 1) >> 1) & 1, sm, status)))
+        return false;
       query_to_f16(sm.q[SM::kQTiles > 1 ? qt : 0], r, q.exponent);
       fence_proxy_async();
       mbar_arrive(&sm.q_f16[qt]);
@@ -670,14 +699,14 @@ chunk_attention_kernel(const ChunkAttention a, int query_blocks) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.k_full[i], 4);
       mbar_init(&sm.v_full[i], 4);
-      mbar_init(&sm.k_empty[i], 1);
-      mbar_init(&sm.v_empty[i], 1);
+      mbar_init(&sm.k_empty[i], w.two ? 2 : 1);      // a tile serves both streams, or one
+      mbar_init(&sm.v_empty[i], w.two ? 2 : 1);
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.p_ready[i], 128);
       mbar_init(&sm.o_done[i], 1);
       mbar_init(&sm.q_f16[i], 128);
     }
-    mbar_init(&sm.all_done, 1);
+    mbar_init(&sm.all_done, 2);
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -708,13 +737,11 @@ chunk_attention_kernel(const ChunkAttention a, int query_blocks) {
     produce(a, sm, w, row, kvh, warp - kProducerWarp0, lane);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == kIssueWarp) {
-      if (lane == 0) {
-        issue(a, sm, w, tmem);
-        // nothing of this CTA's is in flight when its tensor memory goes back, also after an expired wait
-        const unsigned long long t0 = global_ns();
-        while (!mbar_try(&sm.all_done, 0) && global_ns() - t0 < 200000000ull) {}
-      }
+    if (warp < kIssueWarp + 2) {
+      issue(a, sm, w, tmem, warp - kIssueWarp);
+      // nothing of this CTA's is in flight when its tensor memory goes back, also after an expired wait
+      const unsigned long long t0 = global_ns();
+      while (!mbar_try(&sm.all_done, 0) && global_ns() - t0 < 200000000ull) {}
       __syncwarp();
     }
   }
