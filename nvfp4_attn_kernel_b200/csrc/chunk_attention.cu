@@ -49,7 +49,7 @@ struct ChunkSmem {
   uint8_t v[2][kOperandBytes];
   uint8_t raw[RAW][kRawBytes];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_ready[2], o_done[2], q_f16[2], all_done;
+  uint64_t s_full[2], p_ready[2][2], o_done[2], q_f16[2], turn[2], all_done;
   float join[2][128];        // stream 1's maximum and sum, when the streams share a tile
   int tile_valid[8];         // K/V positions of tile t that exist (0: a refused page), at t % 8: the producers are at
                              // most three tiles ahead of the operands, the softmax at most two behind them
@@ -143,6 +143,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
       NVFP4_W8(r, 0), NVFP4_W8(r, 8), NVFP4_W8(r, 16), NVFP4_W8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr), NVFP4_W8(r, 0), NVFP4_W8(r, 8)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -382,21 +388,20 @@ __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Wor
   for (int t = first, u = 0; t < tiles && ok; t += stride, ++u) {
     const bool bf16 = t < w.bf16_tiles;
     ok = mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, sm, status);
-    ok = ok && mbar_wait(&sm.p_ready[s], u & 1, sm, status);
-    if (!__all_sync(kAll, ok)) break;
-    tc_fence_after();
     const uint32_t v = smem_u32(sm.v[t & 1]);
     const uint32_t id = idesc(bf16, bf16);
-    if (bf16) {
-      const uint64_t v_desc = desc_mn_major(v);
+    const uint64_t v_desc = bf16 ? desc_mn_major(v) : desc_k_major(v);
+    const uint32_t step16 = (bf16 ? 2048 : 32) >> 4, step64 = (bf16 ? 4 * 2048 : kHalfBytes) >> 4;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mma_ts(col_o, col_s + i * 8, v_desc + i * (2048 >> 4), id, u > 0 || i > 0, leader);
-    } else {
-      const uint64_t v_desc = desc_k_major(v);
+    for (int half = 0; half < 2; ++half) {      // 64 tokens each: the product starts on the first while the second is computed
+      ok = ok && mbar_wait(&sm.p_ready[s][half], u & 1, sm, status);
+      if (!__all_sync(kAll, ok)) break;
+      tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        mma_ts(col_o, col_s + i * 8, v_desc + (((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4), id, u > 0 || i > 0, leader);
+      for (int i = 0; i < 4; ++i)
+        mma_ts(col_o, col_s + half * 32 + i * 8, v_desc + half * step64 + i * step16, id, u > 0 || half > 0 || i > 0, leader);
     }
+    if (!__all_sync(kAll, ok)) break;
     commit(&sm.o_done[s], leader);
     commit(&sm.v_empty[t & 1], leader);
     if (t + stride < tiles) ok = scores(t + stride);
@@ -478,16 +483,65 @@ __device__ __forceinline__ void query_to_f16(uint8_t* tile, int r, int exponent)
 }
 
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
-  uint32_t b, h;
-  if (bf16) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(hi), "f"(lo));
-    return b;
-  }
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
-  return h;
+  uint32_t v;
+  if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
+}
+
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ uint64_t pair(float v) { return pair(__float_as_uint(v), __float_as_uint(v)); }
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return v;
 }
 
 struct RowState { float m, l; };    // maximum in use (log2 units) and the sum relative to it
+
+// Largest of 64 scores.
+__device__ __forceinline__ float max64(const uint32_t* raw) {
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 64; i += 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top[j] = max3(top[j], raw[i + 2 * j], raw[i + 2 * j + 1]);
+  }
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// 64 scores -> probabilities, packed over the first half of `raw` and stored; their sums are added.
+template <bool BF16>
+__device__ __forceinline__ void exp64(uint32_t* raw, uint64_t scale, uint64_t minus_base, uint64_t (&sum)[2], uint32_t col_p) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    float x, y;
+    unpair(fma2(pair(raw[2 * i], raw[2 * i + 1]), scale, minus_base), x, y);
+    x = ex2(x);
+    y = ex2(y);
+    sum[i & 1] = add2(sum[i & 1], pair(__float_as_uint(x), __float_as_uint(y)));
+    raw[i] = pack16(x, y, BF16);
+  }
+  tmem_st32(col_p, raw);
+}
 
 template <class SM>
 __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int stream, int r,
@@ -504,6 +558,12 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
   const float scale_f16 = fmaxf(a.scale_log2 * exponent_value(q.exponent), 1.2e-38f);
   float m = -INFINITY, l = 0.f;
   const int steps = stream_steps(w, stream);
+  // Two streams over the same tiles compute their exponentials in turns: side by side they would share the
+  // exponential unit, finish together and leave it idle while the tensor cores work for both.
+  auto my_turn = [&](int u) -> bool {
+    if (!w.two || (stream == 0 && u == 0)) return true;
+    return __all_sync(kAll, mbar_wait(&sm.turn[stream], (stream == 0 ? u - 1 : u) & 1, sm, status));
+  };
   for (int u = 0; u < steps; ++u) {
     const int t = w.two ? u : 2 * u + stream, tile = w.begin + t;
     if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream], u & 1, sm, status))) return false;
@@ -521,24 +581,26 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
     }
     if (warp_live) {
       uint32_t raw[128];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(col_s + i * 32, raw + i * 32);
+      tmem_ld32(col_s, raw);
+      tmem_ld32(col_s + 32, raw + 32);
       tmem_ld_wait();
+      tmem_ld32(col_s + 64, raw + 64);
+      tmem_ld32(col_s + 96, raw + 96);
+      const int limit = tile < w.fresh ? q.token - tile * 128 + 1 : sm.tile_valid[t & 7];
+      const bool cut = __any_sync(kAll, limit < 128);
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
+      }
+      float best = max64(raw);
+      tmem_ld_wait();
+      if (cut) {
+#pragma unroll
+        for (int i = 64; i < 128; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
+      }
+      best = fmaxf(best, max64(raw + 64));
       const float scale = bf16 ? scale_bf16 : scale_f16;
       const float offset = tile < w.fresh ? q.shift * scale : 0.f;
-      const int limit = tile < w.fresh ? q.token - tile * 128 + 1 : sm.tile_valid[t & 7];
-      if (__any_sync(kAll, limit < 128)) {
-#pragma unroll
-        for (int i = 0; i < 128; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
-      }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 128; i += 8) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          top[j] = fmaxf(fmaxf(top[j], __uint_as_float(raw[i + 2 * j])), __uint_as_float(raw[i + 2 * j + 1]));
-      }
-      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
       const float now = best == -INFINITY ? -INFINITY : best * scale - offset;
       const bool grows = now > m + kRescaleLog2;
       if (__any_sync(kAll, grows)) {
@@ -546,40 +608,40 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
         if (u > 0) {
           if (!__all_sync(kAll, mbar_wait(&sm.o_done[stream], (u - 1) & 1, sm, status))) return false;
           tc_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            uint32_t o[16];
+            tmem_ld16(col_o + i * 16, o);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t o[32];
-            tmem_ld32(col_o + i * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            tmem_st32(col_o + i * 32, o);
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tmem_st16(col_o + i * 16, o);
           }
         }
         l *= alpha;
         if (grows) m = now;
       }
-      const float base = (m == -INFINITY ? 0.f : m) + offset;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int c = half * 64 + 2 * i;
-          const float x = ex2(fmaf(__uint_as_float(raw[c]), scale, -base));
-          const float y = ex2(fmaf(__uint_as_float(raw[c + 1]), scale, -base));
-          sum[(2 * i) & 3] += x;
-          sum[(2 * i + 1) & 3] += y;
-          p[i] = pack16(x, y, bf16);
-        }
-        tmem_st32(col_s + half * 32, p);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const uint64_t scale2 = pair(scale), minus_base = pair(-((m == -INFINITY ? 0.f : m) + offset));
+      uint64_t sum[2] = {0, 0};
+      if (!my_turn(u)) return false;
+      if (bf16) exp64<true>(raw, scale2, minus_base, sum, col_s);
+      else exp64<false>(raw, scale2, minus_base, sum, col_s);
       tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.p_ready[stream][0]);
+      if (bf16) exp64<true>(raw + 64, scale2, minus_base, sum, col_s + 32);
+      else exp64<false>(raw + 64, scale2, minus_base, sum, col_s + 32);
+      if (w.two) mbar_arrive(&sm.turn[stream ^ 1]);
+      float x, y;
+      unpair(add2(sum[0], sum[1]), x, y);
+      l += x + y;
+      tmem_st_wait();
+    } else {
+      if (!my_turn(u)) return false;
+      if (w.two) mbar_arrive(&sm.turn[stream ^ 1]);
+      mbar_arrive(&sm.p_ready[stream][0]);
     }
     tc_fence_before();
-    mbar_arrive(&sm.p_ready[stream]);
+    mbar_arrive(&sm.p_ready[stream][1]);
   }
   state.m = m;
   state.l = l;
@@ -702,7 +764,9 @@ chunk_attention_kernel(const ChunkAttention a, int query_blocks) {
       mbar_init(&sm.k_empty[i], w.two ? 2 : 1);      // a tile serves both streams, or one
       mbar_init(&sm.v_empty[i], w.two ? 2 : 1);
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_ready[i], 128);
+      mbar_init(&sm.p_ready[i][0], 128);
+      mbar_init(&sm.p_ready[i][1], 128);
+      mbar_init(&sm.turn[i], 128);
       mbar_init(&sm.o_done[i], 1);
       mbar_init(&sm.q_f16[i], 128);
     }
