@@ -33,6 +33,7 @@ using namespace sm100;
 constexpr int kThreads = 512;         // two softmax warpgroups, the producers, the issuer's warpgroup
 constexpr int kProducerWarp0 = 8;
 constexpr int kIssueWarp = 12;        // and 13: one per stream
+constexpr int kFetchWarp = 14;        // page bytes
 constexpr int kOperandBytes = 128 * 256;       // 128 rows of 128 16-bit elements: two 128-byte swizzled halves
 constexpr int kHalfBytes = 128 * 128;
 constexpr int kRawBytes = 8192 + 1024;         // a page's nibbles and scales for one head
@@ -49,7 +50,8 @@ struct ChunkSmem {
   uint8_t v[2][kOperandBytes];
   uint8_t raw[RAW][kRawBytes];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_ready[2][2], o_done[2], q_f16[2], turn[2], all_done;
+  uint64_t s_full[2][2], p_ready[2][2], o_done[2], q_f16[2], all_done;
+  uint64_t raw_full[RAW], raw_empty[RAW];
   float join[2][128];        // stream 1's maximum and sum, when the streams share a tile
   int tile_valid[8];         // K/V positions of tile t that exist (0: a refused page), at t % 8: the producers are at
                              // most three tiles ahead of the operands, the softmax at most two behind them
@@ -65,22 +67,13 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
   const uint32_t bytes = valid ? 16 : 0;     // 0: the destination is zero-filled
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void cp_async_wait_most(int pending) {   // at most `pending` groups left in flight
-  switch (pending) {
-    case 0: cp_async_wait<0>(); break;
-    case 1: cp_async_wait<1>(); break;
-    case 2: cp_async_wait<2>(); break;
-    case 3: cp_async_wait<3>(); break;
-    case 4: cp_async_wait<4>(); break;
-    case 5: cp_async_wait<5>(); break;
-    default: cp_async_wait<6>(); break;
-  }
+__device__ __forceinline__ void cp_async_wait_most(int pending) {   // at most `pending` groups (0 to 2) left in flight
+  if (pending == 0) cp_async_wait<0>();
+  else if (pending == 1) cp_async_wait<1>();
+  else cp_async_wait<2>();
 }
 
 // Descriptors of a 16-bit operand tile, 128-byte swizzle, eight-row groups 1024 bytes apart.  K-major:
@@ -94,10 +87,10 @@ __device__ __forceinline__ uint64_t desc_mn_major(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(kHalfBytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// M = 128, N = 128, fp32 accumulators; A and B both FP16 (0) or both BF16 (1)
-__device__ __forceinline__ uint32_t idesc(bool bf16, bool b_mn_major) {
+// M = 128, fp32 accumulators; A and B both FP16 or both BF16
+__device__ __forceinline__ uint32_t idesc(bool bf16, bool b_mn_major, uint32_t n) {
   const uint32_t f = bf16 ? 1u : 0u;
-  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
 // Issued by the lane whose `leader` is set, out of a warp that runs converged.
@@ -182,6 +175,9 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   return r;
 }
 
+// Tensor maps of the packed page regions.
+struct ChunkMaps { CUtensorMap k, v; };
+
 // What a CTA works on.
 struct Work {
   ChunkRow r;
@@ -216,24 +212,19 @@ __device__ __forceinline__ uint4 bf16x8_to_f16x8(const uint4& v, float f) {
 
 // -- producers -----------------------------------------------------------------------------------
 
-// Items of K/V work in order: 2 t = K of tile t, 2 t + 1 = V of tile t (t from the split's first tile).
+// Items of K/V work in order: K0, then K1 V0, K2 V1, ... and the last V: K runs a tile ahead of V, because an issuer
+// forms the next scores of its stream between the two halves of a tile's P V.
+struct Item { int t; bool is_v; };
+__device__ __forceinline__ Item item_of(int i, int items) {
+  if (i == items - 1) return {(items >> 1) - 1, true};
+  return (i & 1) ? Item{(i + 1) >> 1, false} : i == 0 ? Item{0, false} : Item{(i >> 1) - 1, true};
+}
 template <class SM>
 struct Producer {
   const ChunkAttention& a;
   SM& sm;
   const Work& w;
-  int row, kvh, warp, lane;
-  int page_base = -1;       // first of the 32 page-table entries that the lanes hold
-  int page_mine = 0;
-
-  __device__ __forceinline__ int64_t page_of(int p) {
-    if (page_base < 0 || p >= page_base + 32) {
-      page_base = p;
-      const int at = p + lane;
-      page_mine = at < w.r.pages ? a.c.page_table[(int64_t)row * a.c.page_table_row_stride + at] : -1;
-    }
-    return __shfl_sync(0xffffffffu, page_mine, p - page_base);
-  }
+  int kvh, warp, lane;
 
   // 128 tokens of BF16 rows straight into an operand tile
   __device__ __forceinline__ void issue_bf16(int tile, bool is_v, uint32_t dst) {
@@ -260,43 +251,25 @@ struct Producer {
     if (!is_v && warp == 0 && lane == 0) sm.tile_valid[(tile - w.begin) & 7] = valid;
   }
 
-  // this warp's 32 rows of a page's nibbles and scales into a raw slot
-  __device__ __forceinline__ void issue_page(int tile, bool is_v, uint8_t* slot) {
-    const ChunkCache& c = a.c;
-    const int64_t page = page_of(tile - w.fresh - w.tail_tiles);
-    const bool ok = page >= 0 && page < c.num_pages;
-    if (!is_v && warp == 0 && lane == 0) {
-      sm.tile_valid[(tile - w.begin) & 7] = ok ? 128 : 0;
-      if (!ok) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
-    }
-    const int64_t at = ok ? page : 0;
-    const uint8_t* packed = is_v ? c.v_packed + at * c.v_pitch + (int64_t)kvh * 8192 : c.k_packed + at * c.k_pitch + kvh * 64;
-    const uint8_t* scales = (is_v ? c.v_sf + at * c.v_sf_pitch : c.k_sf + at * c.k_sf_pitch) + kvh * kSfBlockBytes;
-    const int64_t stride = is_v ? 64 : (int64_t)c.heads_kv * 64;
-    const uint32_t dst = smem_u32(slot);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = warp * 32 + i * 8 + (lane >> 2), piece = lane & 3;
-      cp_async16(dst + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4), packed + r * stride + piece * 16, ok);
-    }
-    if (ok) {
-      cp_async4(dst + 8192 + warp * 256 + lane * 8, scales + lane * 16 + warp * 4);
-      cp_async4(dst + 8192 + warp * 256 + lane * 8 + 4, scales + 512 + lane * 16 + warp * 4);
-    } else {      // a refused page: zeros everywhere, its scores are masked
-      *reinterpret_cast<uint2*>(slot + 8192 + warp * 256 + lane * 8) = make_uint2(0, 0);
-    }
-  }
-
-  // row warp * 32 + lane of a raw slot, dequantised into an operand tile
-  __device__ __forceinline__ void expand(const uint8_t* slot, uint8_t* dst) {
+  // row warp * 32 + lane of a raw slot (the fetch's 64-byte swizzle undone), dequantised into an operand tile; a
+  // refused page: zeros (its scores are masked)
+  __device__ __forceinline__ void expand(const uint8_t* slot, uint8_t* dst, bool valid) {
     const int r = warp * 32 + lane;
-    const uint2 s = *reinterpret_cast<const uint2*>(slot + 8192 + warp * 256 + lane * 8);
+    const uint8_t* scales = slot + 8192 + lane * 16 + warp * 4;
+    const uint32_t s[2] = {*reinterpret_cast<const uint32_t*>(scales), *reinterpret_cast<const uint32_t*>(scales + 512)};
+    uint4 n[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) n[p] = *reinterpret_cast<const uint4*>(slot + r * 64 + ((p ^ ((r >> 1) & 3)) << 4));
+    if (!valid) {
+#pragma unroll
+      for (int p = 0; p < 16; ++p) *reinterpret_cast<uint4*>(dst + swizzled(r, p)) = make_uint4(0, 0, 0, 0);
+      return;
+    }
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      const uint4 n = *reinterpret_cast<const uint4*>(slot + r * 64 + ((p ^ ((r >> 1) & 3)) << 4));
-      const uint32_t two = e4m3x2_to_f16x2(((p & 2) ? s.y : s.x) >> ((p & 1) * 16));
+      const uint32_t two = e4m3x2_to_f16x2(s[p >> 1] >> ((p & 1) * 16));
       const uint32_t s0 = __byte_perm(two, two, 0x1010), s1 = __byte_perm(two, two, 0x3232);
-      const uint32_t words[4] = {n.x, n.y, n.z, n.w};
+      const uint32_t words[4] = {n[p].x, n[p].y, n[p].z, n[p].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t h[4];
@@ -309,41 +282,91 @@ struct Producer {
   }
 };
 
+// Page bytes, in the order of the items, up to RAW of them ahead of their expansion: one tensor copy of the head's
+// 128 x 64 bytes and one bulk copy of its scales each.  Page ids are fetched 32 at a time.
 template <class SM>
-__device__ __forceinline__ void produce(const ChunkAttention& a, SM& sm, const Work& w, int row, int kvh, int warp, int lane) {
+__device__ __forceinline__ void fetch(const ChunkAttention& a, const ChunkMaps& maps, SM& sm, const Work& w, int row, int kvh,
+                                      int lane) {
   constexpr int RAW = SM::kRaw;
-  Producer<SM> p{a, sm, w, row, kvh, warp, lane};
-  const int items = 2 * (w.end - w.begin), first_page_item = 2 * w.bf16_tiles;
-  int issued = 0;
+  constexpr uint32_t kAll = 0xffffffffu;
+  const ChunkCache& c = a.c;
+  const int items = 2 * (w.end - w.begin), first_page = w.begin + w.bf16_tiles - w.fresh - w.tail_tiles;
+  const int32_t* table = c.page_table + (int64_t)row * c.page_table_row_stride + first_page;
+  const int pages = w.end - w.begin - w.bf16_tiles;
+  int held[2] = {-1, -1}, ids[2] = {0, 0};       // K and V are a tile apart: 32 ids each
+  int j = 0;
   for (int item = 0; item < items; ++item) {
-    // Issue ahead: BF16 items go straight into an operand stage, two items (the next tile's same operand) ahead,
-    // once that stage is empty; a third would wait for products that wait for this item.  Page items go into the
-    // raw slot that the item RAW before them has left.
-    while (issued < items && (issued < first_page_item ? issued <= item + 2 : issued < item + RAW)) {
-      const int t = issued >> 1;
-      const bool is_v = issued & 1;
-      if (issued < first_page_item) {
-        if (t >= 2 && !mbar_wait(is_v ? &sm.v_empty[t & 1] : &sm.k_empty[t & 1], ((t >> 1) - 1) & 1, sm, a.c.status)) goto out;
-        p.issue_bf16(w.begin + t, is_v, smem_u32(is_v ? sm.v[t & 1] : sm.k[t & 1]));
+    const Item n = item_of(item, items);
+    if (n.t < w.bf16_tiles) continue;
+    const int p = n.t - w.bf16_tiles, slot = j % RAW;
+    if (held[n.is_v] != p >> 5) {
+      held[n.is_v] = p >> 5;
+      const int at = (p & ~31) + lane;
+      ids[n.is_v] = at < pages ? table[at] : -1;
+    }
+    const int64_t page = __shfl_sync(kAll, ids[n.is_v], p & 31);
+    const bool ok = page >= 0 && page < c.num_pages;
+    if (j >= RAW && !__all_sync(kAll, mbar_wait(&sm.raw_empty[slot], (j / RAW - 1) & 1, sm, c.status))) break;
+    if (lane == 0) {
+      if (!n.is_v) {
+        sm.tile_valid[n.t & 7] = ok ? 128 : 0;
+        if (!ok) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
+      }
+      if (ok) {
+        mbar_expect_tx(&sm.raw_full[slot], kRawBytes);
+        const uint32_t dst = smem_u32(sm.raw[slot]);
+        if (n.is_v) tma_load_4d(dst, &maps.v, &sm.raw_full[slot], 0, 0, kvh, (int)page);
+        else tma_load_4d(dst, &maps.k, &sm.raw_full[slot], 0, kvh, 0, (int)page);
+        bulk_load(dst + 8192, (n.is_v ? c.v_sf + page * c.v_sf_pitch : c.k_sf + page * c.k_sf_pitch) + kvh * kSfBlockBytes,
+                  kSfBlockBytes, &sm.raw_full[slot]);
       } else {
-        p.issue_page(w.begin + t, is_v, sm.raw[issued % RAW]);
+        mbar_arrive(&sm.raw_full[slot]);
       }
-      cp_async_commit();
-      ++issued;
     }
-    cp_async_wait_most(issued - item - 1);
     __syncwarp();
-    {
-      const int t = item >> 1;
-      const bool is_v = item & 1;
-      if (item >= first_page_item) {
-        if (t >= 2 && !mbar_wait(is_v ? &sm.v_empty[t & 1] : &sm.k_empty[t & 1], ((t >> 1) - 1) & 1, sm, a.c.status)) goto out;
-        p.expand(sm.raw[item % RAW], is_v ? sm.v[t & 1] : sm.k[t & 1]);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(is_v ? &sm.v_full[t & 1] : &sm.k_full[t & 1]);
+    ++j;
+  }
+  // nothing lands in shared memory after the CTA is gone, also after an expired wait
+  const unsigned long long t0 = global_ns();
+  for (int k = j > RAW ? j - RAW : 0; k < j; ++k)
+    while (!mbar_try(&sm.raw_full[k % RAW], (k / RAW) & 1) && global_ns() - t0 < 200000000ull) {}
+}
+
+template <class SM>
+__device__ __forceinline__ void produce(const ChunkAttention& a, SM& sm, const Work& w, int kvh, int warp, int lane) {
+  constexpr int RAW = SM::kRaw;
+  Producer<SM> p{a, sm, w, kvh, warp, lane};
+  const int items = 2 * (w.end - w.begin);
+  auto empty = [&](const Item& n) -> bool {       // the operand stage of the tile before last has been used
+    return n.t < 2 || mbar_wait(n.is_v ? &sm.v_empty[n.t & 1] : &sm.k_empty[n.t & 1], ((n.t >> 1) - 1) & 1, sm, a.c.status);
+  };
+  int next = 0, in_flight = 0, j = 0;     // first item not looked at, BF16 items issued and not landed, page items so far
+  for (int item = 0; item < items; ++item) {
+    // BF16 items go straight into an operand stage, two items ahead at most (the last V one: it follows its own K
+    // at two), once that stage is empty - what frees it must not wait for an item that is not through here yet.
+    // (Their last one is V of tile bf16_tiles - 1, item 2 * bf16_tiles at most.)
+    for (; next <= 2 * w.bf16_tiles && next < items && next <= item + (next == items - 1 ? 1 : 2); ++next) {
+      const Item n = item_of(next, items);
+      if (n.t >= w.bf16_tiles) continue;
+      if (!empty(n)) goto out;
+      p.issue_bf16(w.begin + n.t, n.is_v, smem_u32(n.is_v ? sm.v[n.t & 1] : sm.k[n.t & 1]));
+      cp_async_commit();
+      ++in_flight;
     }
+    const Item n = item_of(item, items);
+    if (n.t < w.bf16_tiles) {
+      cp_async_wait_most(--in_flight);
+    } else {
+      const int slot = j % RAW;
+      if (!mbar_wait(&sm.raw_full[slot], (j / RAW) & 1, sm, a.c.status) || !empty(n)) goto out;
+      p.expand(sm.raw[slot], n.is_v ? sm.v[n.t & 1] : sm.k[n.t & 1], sm.tile_valid[n.t & 7] != 0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.raw_empty[slot]);
+      ++j;
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(n.is_v ? &sm.v_full[n.t & 1] : &sm.k_full[n.t & 1]);
   }
 out:
   cp_async_wait<0>();
@@ -351,9 +374,11 @@ out:
 
 // -- issuers -------------------------------------------------------------------------------------
 
-// One warp per stream: scores of tile t, then, step by step, P V of a tile and the scores of the next one (which
-// overwrite the tensor-memory columns that P sat in; the products of one thread complete in order).  The whole warp
-// runs the loop, so addresses and descriptors stay in uniform registers; one elected lane issues.
+// One warp per stream.  A tile's 128 tokens go through tensor memory as two halves of 64 columns: scores of a
+// half, its probabilities over the same columns, P V, scores of the next tile's half - so that the softmax
+// always has one half to work on while the tensor cores turn the other around (the products of one thread
+// complete in order).  The whole warp runs the loop, so addresses and descriptors stay in uniform registers; one
+// elected lane issues.
 template <class SM>
 __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int s) {
   constexpr uint32_t kAll = 0xffffffffu;
@@ -364,47 +389,47 @@ __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Wor
   const uint64_t q_desc = desc_k_major(smem_u32(sm.q[SM::kQTiles > 1 ? qt : 0]));
   const uint32_t col_s = tmem + kColS + s * 128, col_o = tmem + kColO + s * 128;
   bool f16_seen = w.bf16_tiles == 0;
-  auto scores = [&](int t) -> bool {
+  auto scores = [&](int t, int half) -> bool {
     const bool bf16 = t < w.bf16_tiles;
-    bool ok = mbar_wait(&sm.k_full[t & 1], (t >> 1) & 1, sm, status);
-    if (!bf16 && !f16_seen) {
-      ok = ok && mbar_wait(&sm.q_f16[qt], 0, sm, status);
-      f16_seen = true;
+    if (half == 0) {
+      bool ok = mbar_wait(&sm.k_full[t & 1], (t >> 1) & 1, sm, status);
+      if (!bf16 && !f16_seen) {
+        ok = ok && mbar_wait(&sm.q_f16[qt], 0, sm, status);
+        f16_seen = true;
+      }
+      if (!__all_sync(kAll, ok)) return false;
+      tc_fence_after();
     }
-    if (!__all_sync(kAll, ok)) return false;
-    tc_fence_after();
-    const uint64_t k_desc = desc_k_major(smem_u32(sm.k[t & 1]));
-    const uint32_t id = idesc(bf16, false);
+    const uint64_t k_desc = desc_k_major(smem_u32(sm.k[t & 1]) + half * (kHalfBytes / 2));
+    const uint32_t id = idesc(bf16, false, 64);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint64_t at = ((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4;
-      mma_ss(col_s, q_desc + at, k_desc + at, id, i > 0, leader);
+      mma_ss(col_s + half * 64, q_desc + at, k_desc + at, id, i > 0, leader);
     }
-    commit(&sm.s_full[s], leader);
-    commit(&sm.k_empty[t & 1], leader);
+    commit(&sm.s_full[s][half], leader);
+    if (half) commit(&sm.k_empty[t & 1], leader);
     return true;
   };
-  bool ok = first < tiles && scores(first);
+  bool ok = first < tiles && scores(first, 0) && scores(first, 1);
   for (int t = first, u = 0; t < tiles && ok; t += stride, ++u) {
     const bool bf16 = t < w.bf16_tiles;
     ok = mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, sm, status);
     const uint32_t v = smem_u32(sm.v[t & 1]);
-    const uint32_t id = idesc(bf16, bf16);
+    const uint32_t id = idesc(bf16, bf16, 128);
     const uint64_t v_desc = bf16 ? desc_mn_major(v) : desc_k_major(v);
     const uint32_t step16 = (bf16 ? 2048 : 32) >> 4, step64 = (bf16 ? 4 * 2048 : kHalfBytes) >> 4;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {      // 64 tokens each: the product starts on the first while the second is computed
+    for (int half = 0; half < 2; ++half) {
       ok = ok && mbar_wait(&sm.p_ready[s][half], u & 1, sm, status);
-      if (!__all_sync(kAll, ok)) break;
+      if (!__all_sync(kAll, ok)) { ok = false; break; }
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        mma_ts(col_o, col_s + half * 32 + i * 8, v_desc + half * step64 + i * step16, id, u > 0 || half > 0 || i > 0, leader);
+        mma_ts(col_o, col_s + half * 64 + i * 8, v_desc + half * step64 + i * step16, id, u > 0 || half > 0 || i > 0, leader);
+      commit(&sm.o_done[s], leader);
+      if (half) commit(&sm.v_empty[t & 1], leader);
+      if (t + stride < tiles && !scores(t + stride, half)) { ok = false; break; }
     }
-    if (!__all_sync(kAll, ok)) break;
-    commit(&sm.o_done[s], leader);
-    commit(&sm.v_empty[t & 1], leader);
-    if (t + stride < tiles) ok = scores(t + stride);
   }
   commit(&sm.all_done, leader);
 }
@@ -558,90 +583,72 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
   const float scale_f16 = fmaxf(a.scale_log2 * exponent_value(q.exponent), 1.2e-38f);
   float m = -INFINITY, l = 0.f;
   const int steps = stream_steps(w, stream);
-  // Two streams over the same tiles compute their exponentials in turns: side by side they would share the
-  // exponential unit, finish together and leave it idle while the tensor cores work for both.
-  auto my_turn = [&](int u) -> bool {
-    if (!w.two || (stream == 0 && u == 0)) return true;
-    return __all_sync(kAll, mbar_wait(&sm.turn[stream], (stream == 0 ? u - 1 : u) & 1, sm, status));
-  };
   for (int u = 0; u < steps; ++u) {
     const int t = w.two ? u : 2 * u + stream, tile = w.begin + t;
-    if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream], u & 1, sm, status))) return false;
-    tc_fence_after();
     const bool bf16 = t < w.bf16_tiles;
-    if (t == w.bf16_tiles - 1 && w.bf16_tiles < w.end - w.begin) {
-      // the last product with the BF16 query: once the other stream's is done too where they share it (its next
-      // one waits for what follows), the rows become FP16
-      if (!w.two && t > 0 &&
-          !__all_sync(kAll, mbar_wait(&sm.s_full[stream ^ 1], ((t - 1) >> 1) & 1, sm, status)))
-        return false;
-      query_to_f16(sm.q[SM::kQTiles > 1 ? qt : 0], r, q.exponent);
-      fence_proxy_async();
-      mbar_arrive(&sm.q_f16[qt]);
-    }
-    if (warp_live) {
-      uint32_t raw[128];
-      tmem_ld32(col_s, raw);
-      tmem_ld32(col_s + 32, raw + 32);
-      tmem_ld_wait();
-      tmem_ld32(col_s + 64, raw + 64);
-      tmem_ld32(col_s + 96, raw + 96);
-      const int limit = tile < w.fresh ? q.token - tile * 128 + 1 : sm.tile_valid[t & 7];
-      const bool cut = __any_sync(kAll, limit < 128);
-      if (cut) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
-      }
-      float best = max64(raw);
-      tmem_ld_wait();
-      if (cut) {
-#pragma unroll
-        for (int i = 64; i < 128; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
-      }
-      best = fmaxf(best, max64(raw + 64));
-      const float scale = bf16 ? scale_bf16 : scale_f16;
-      const float offset = tile < w.fresh ? q.shift * scale : 0.f;
-      const float now = best == -INFINITY ? -INFINITY : best * scale - offset;
-      const bool grows = now > m + kRescaleLog2;
-      if (__any_sync(kAll, grows)) {
-        const float alpha = grows ? ex2(m - now) : 1.f;       // 0 from an empty row
-        if (u > 0) {
-          if (!__all_sync(kAll, mbar_wait(&sm.o_done[stream], (u - 1) & 1, sm, status))) return false;
-          tc_fence_after();
+    const float scale = bf16 ? scale_bf16 : scale_f16;
+    const float offset = tile < w.fresh ? q.shift * scale : 0.f;
+    int limit = 128;
 #pragma unroll 1
-          for (int i = 0; i < 8; ++i) {
-            uint32_t o[16];
-            tmem_ld16(col_o + i * 16, o);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            tmem_st16(col_o + i * 16, o);
-          }
+    for (int half = 0; half < 2; ++half) {
+      if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream][half], u & 1, sm, status))) return false;
+      tc_fence_after();
+      if (half == 0) {
+        limit = tile < w.fresh ? q.token - tile * 128 + 1 : sm.tile_valid[t & 7];
+      } else {
+        limit -= 64;
+        if (t == w.bf16_tiles - 1 && w.bf16_tiles < w.end - w.begin) {
+          // the last product with the BF16 query: once the other stream's is done too where they share it (its next
+          // one waits for what follows), the rows become FP16
+          if (!w.two && t > 0 &&
+              !__all_sync(kAll, mbar_wait(&sm.s_full[stream ^ 1][1], ((t - 1) >> 1) & 1, sm, status)))
+            return false;
+          query_to_f16(sm.q[SM::kQTiles > 1 ? qt : 0], r, q.exponent);
+          fence_proxy_async();
+          mbar_arrive(&sm.q_f16[qt]);
         }
-        l *= alpha;
-        if (grows) m = now;
       }
-      const uint64_t scale2 = pair(scale), minus_base = pair(-((m == -INFINITY ? 0.f : m) + offset));
-      uint64_t sum[2] = {0, 0};
-      if (!my_turn(u)) return false;
-      if (bf16) exp64<true>(raw, scale2, minus_base, sum, col_s);
-      else exp64<false>(raw, scale2, minus_base, sum, col_s);
-      tmem_st_wait();
+      if (warp_live) {
+        uint32_t raw[64];
+        tmem_ld32(col_s + half * 64, raw);
+        tmem_ld32(col_s + half * 64 + 32, raw + 32);
+        tmem_ld_wait();
+        if (__any_sync(kAll, limit < 64)) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
+        }
+        const float best = max64(raw);
+        const float now = best == -INFINITY ? -INFINITY : best * scale - offset;
+        const bool grows = now > m + kRescaleLog2;
+        if (__any_sync(kAll, grows)) {
+          const float alpha = grows ? ex2(m - now) : 1.f;       // 0 from an empty row
+          if (u > 0 || half > 0) {      // every product so far has to be in O: the last one is half-step 2 u + half - 1
+            if (!__all_sync(kAll, mbar_wait(&sm.o_done[stream], (half + 1) & 1, sm, status))) return false;
+            tc_fence_after();
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              uint32_t o[16];
+              tmem_ld16(col_o + i * 16, o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+              tmem_st16(col_o + i * 16, o);
+            }
+          }
+          l *= alpha;
+          if (grows) m = now;
+        }
+        const uint64_t scale2 = pair(scale), minus_base = pair(-((m == -INFINITY ? 0.f : m) + offset));
+        uint64_t sum[2] = {0, 0};
+        if (bf16) exp64<true>(raw, scale2, minus_base, sum, col_s + half * 64);
+        else exp64<false>(raw, scale2, minus_base, sum, col_s + half * 64);
+        float x, y;
+        unpair(add2(sum[0], sum[1]), x, y);
+        l += x + y;
+        tmem_st_wait();
+      }
       tc_fence_before();
-      mbar_arrive(&sm.p_ready[stream][0]);
-      if (bf16) exp64<true>(raw + 64, scale2, minus_base, sum, col_s + 32);
-      else exp64<false>(raw + 64, scale2, minus_base, sum, col_s + 32);
-      if (w.two) mbar_arrive(&sm.turn[stream ^ 1]);
-      float x, y;
-      unpair(add2(sum[0], sum[1]), x, y);
-      l += x + y;
-      tmem_st_wait();
-    } else {
-      if (!my_turn(u)) return false;
-      if (w.two) mbar_arrive(&sm.turn[stream ^ 1]);
-      mbar_arrive(&sm.p_ready[stream][0]);
+      mbar_arrive(&sm.p_ready[stream][half]);
     }
-    tc_fence_before();
-    mbar_arrive(&sm.p_ready[stream][1]);
   }
   state.m = m;
   state.l = l;
@@ -726,7 +733,7 @@ __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Wo
 // grid (query blocks * splits, heads_kv, rows)
 template <int QTILES, int RAW>
 __global__ void __launch_bounds__(kThreads, 1)
-chunk_attention_kernel(const ChunkAttention a, int query_blocks) {
+chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps maps, int query_blocks) {
   using SM = ChunkSmem<QTILES, RAW>;
   extern __shared__ uint8_t smem_raw[];
   SM& sm = *reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -763,14 +770,18 @@ chunk_attention_kernel(const ChunkAttention a, int query_blocks) {
       mbar_init(&sm.v_full[i], 4);
       mbar_init(&sm.k_empty[i], w.two ? 2 : 1);      // a tile serves both streams, or one
       mbar_init(&sm.v_empty[i], w.two ? 2 : 1);
-      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.s_full[i][0], 1);
+      mbar_init(&sm.s_full[i][1], 1);
       mbar_init(&sm.p_ready[i][0], 128);
       mbar_init(&sm.p_ready[i][1], 128);
-      mbar_init(&sm.turn[i], 128);
       mbar_init(&sm.o_done[i], 1);
       mbar_init(&sm.q_f16[i], 128);
     }
     mbar_init(&sm.all_done, 2);
+    for (int i = 0; i < RAW; ++i) {
+      mbar_init(&sm.raw_full[i], 1);
+      mbar_init(&sm.raw_empty[i], 4);
+    }
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -798,7 +809,7 @@ chunk_attention_kernel(const ChunkAttention a, int query_blocks) {
     finish(a, sm, w, tmem, stream, r, q, state, split, ok);
   } else if (stream == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    produce(a, sm, w, row, kvh, warp - kProducerWarp0, lane);
+    produce(a, sm, w, kvh, warp - kProducerWarp0, lane);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp < kIssueWarp + 2) {
@@ -807,6 +818,8 @@ chunk_attention_kernel(const ChunkAttention a, int query_blocks) {
       const unsigned long long t0 = global_ns();
       while (!mbar_try(&sm.all_done, 0) && global_ns() - t0 < 200000000ull) {}
       __syncwarp();
+    } else if (warp == kFetchWarp) {
+      fetch(a, maps, sm, w, row, kvh, lane);
     }
   }
   tc_fence_before();
@@ -853,9 +866,15 @@ cudaError_t launch(const ChunkAttention& a, cudaStream_t stream) {
   static_assert(sizeof(ChunkSmem<QTILES, RAW>) + 1024 <= 232448, "shared memory of one CTA");
   cudaError_t e = cudaFuncSetAttribute(chunk_attention_kernel<QTILES, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
+  ChunkMaps maps{};
+  if (a.c.max_pages > 0 && a.c.num_pages > 0) {
+    e = encode_map(0, a.c.k_packed, a.c.k_pitch, a.c.num_pages, a.c.heads_kv, &maps.k);
+    if (e == cudaSuccess) e = encode_map(1, a.c.v_packed, a.c.v_pitch, a.c.num_pages, a.c.heads_kv, &maps.v);
+    if (e != cudaSuccess) return e;
+  }
   const int tokens = 128 / (a.heads_q / a.c.heads_kv) * QTILES;
   const int blocks = (a.c.max_chunk + tokens - 1) / tokens;
-  chunk_attention_kernel<QTILES, RAW><<<dim3(blocks * a.num_splits, a.c.heads_kv, a.c.rows), kThreads, bytes, stream>>>(a, blocks);
+  chunk_attention_kernel<QTILES, RAW><<<dim3(blocks * a.num_splits, a.c.heads_kv, a.c.rows), kThreads, bytes, stream>>>(a, maps, blocks);
   return cudaGetLastError();
 }
 

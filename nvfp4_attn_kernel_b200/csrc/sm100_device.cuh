@@ -275,22 +275,8 @@ struct MapEntry { MapKey key; CUtensorMap map; bool valid; };
 // K: bytes [64] x heads x tokens [128] x pages ; V: bytes [64] x channels [128] x heads x pages ;
 // which = 2: a BF16 tail cache (pitch unused)
 constexpr int kTailBoxRows = 32;   // tokens per box of a tail map
-inline cudaError_t make_map(int which, const void* base, int64_t pitch, int64_t pages, int heads,
-                            CUtensorMap* out) {
-  // four maps per launch (K, V and the two tail caches) and one set per layer of a model: a
-  // direct-mapped cache by address, so that an eager step does not encode maps at every call
-  constexpr int kCached = 256;
-  thread_local MapEntry cache[kCached] = {};
-  const MapKey key{base, pitch, pages, heads, which};
-  const unsigned long long h =
-      (static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(base)) + (unsigned long long)which) *
-      0x9E3779B97F4A7C15ull;
-  // two candidate places per key: the maps of one launch rarely push each other out
-  MapEntry* slot = &cache[(h >> 56) % kCached];
-  if (slot->valid && slot->key == key) { *out = slot->map; return cudaSuccess; }
-  MapEntry* second = &cache[((h >> 48) ^ 0x55u) % kCached];
-  if (second->valid && second->key == key) { *out = second->map; return cudaSuccess; }
-  if (slot->valid && !second->valid) slot = second;
+inline cudaError_t encode_map(int which, const void* base, int64_t pitch, int64_t pages, int heads,
+                              CUtensorMap* out) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return cudaErrorNotSupported;
   cuuint64_t dims[4], strides[3];
@@ -312,11 +298,32 @@ inline cudaError_t make_map(int which, const void* base, int64_t pitch, int64_t 
     box[0] = 128; box[1] = 1; box[2] = kTailBoxRows; box[3] = 1;
   }
   CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
-  CUtensorMap map;
-  CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, which >= 2 ? 3 : 4, const_cast<void*>(base), dims, strides, box, estr,
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, which >= 2 ? 3 : 4, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, which >= 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                   promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
+  return cudaSuccess;
+}
+
+inline cudaError_t make_map(int which, const void* base, int64_t pitch, int64_t pages, int heads,
+                            CUtensorMap* out) {
+  // four maps per launch (K, V and the two tail caches) and one set per layer of a model: a
+  // direct-mapped cache by address, so that an eager step does not encode maps at every call
+  constexpr int kCached = 256;
+  thread_local MapEntry cache[kCached] = {};
+  const MapKey key{base, pitch, pages, heads, which};
+  const unsigned long long h =
+      (static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(base)) + (unsigned long long)which) *
+      0x9E3779B97F4A7C15ull;
+  // two candidate places per key: the maps of one launch rarely push each other out
+  MapEntry* slot = &cache[(h >> 56) % kCached];
+  if (slot->valid && slot->key == key) { *out = slot->map; return cudaSuccess; }
+  MapEntry* second = &cache[((h >> 48) ^ 0x55u) % kCached];
+  if (second->valid && second->key == key) { *out = second->map; return cudaSuccess; }
+  if (slot->valid && !second->valid) slot = second;
+  CUtensorMap map;
+  cudaError_t e = encode_map(which, base, pitch, pages, heads, &map);
+  if (e != cudaSuccess) return e;
   *slot = MapEntry{key, map, true};
   *out = map;
   return cudaSuccess;
