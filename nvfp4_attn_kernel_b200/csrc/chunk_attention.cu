@@ -30,10 +30,9 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kThreads = 512;         // two softmax warpgroups, the producers, the issuer's warpgroup
-constexpr int kProducerWarp0 = 8;
-constexpr int kIssueWarp = 12;        // and 13: one per stream
-constexpr int kFetchWarp = 14;        // page bytes
+constexpr int kThreads = 640;         // warpgroups: softmax of two streams, K operands, V operands, issuers and fetch
+constexpr int kIssueWarp = 16;        // and 17: one per stream
+constexpr int kFetchWarp = 18;        // page bytes
 constexpr int kOperandBytes = 128 * 256;       // 128 rows of 128 16-bit elements: two 128-byte swizzled halves
 constexpr int kHalfBytes = 128 * 128;
 constexpr int kRawBytes = 8192 + 1024;         // a page's nibbles and scales for one head
@@ -41,20 +40,21 @@ constexpr float kRescaleLog2 = 8.f;
 constexpr uint32_t kColS = 0, kColO = 256;     // tensor-memory columns of stream 0; stream 1: + 128
 constexpr float kLn2 = 0.6931471805599453f;
 
-// QTILES query tiles in shared memory, RAW slots of page bytes in flight
+// QTILES query tiles in shared memory, RAW slots of page bytes in flight, RAWK of them for K.  (A ring per operand: a
+// waiter on a slot's barrier has to have seen each of its phases, and loads do not land in the order of their issue.)
 template <int QTILES, int RAW>
 struct ChunkSmem {
-  static constexpr int kQTiles = QTILES, kRaw = RAW;
+  static constexpr int kQTiles = QTILES, kRaw = RAW, kRawK = (RAW + 1) / 2, kRawV = RAW - kRawK;
   uint8_t q[QTILES][kOperandBytes];
   uint8_t k[2][kOperandBytes];
   uint8_t v[2][kOperandBytes];
   uint8_t raw[RAW][kRawBytes];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2][2], p_ready[2][2], o_done[2], q_f16[2], all_done;
+  uint64_t q_ready[2], q_f16[2], s_full[2][2], p_ready[2][2], o_done[2], all_done;
   uint64_t raw_full[RAW], raw_empty[RAW];
   float join[2][128];        // stream 1's maximum and sum, when the streams share a tile
-  int tile_valid[8];         // K/V positions of tile t that exist (0: a refused page), at t % 8: the producers are at
-                             // most three tiles ahead of the operands, the softmax at most two behind them
+  int page_ok[8];            // whether page tile t was fetched (0: a refused id), at t % 8: the fetch is at most six
+                             // tiles ahead of the softmax
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -70,12 +70,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void cp_async_wait_most(int pending) {   // at most `pending` groups (0 to 2) left in flight
-  if (pending == 0) cp_async_wait<0>();
-  else if (pending == 1) cp_async_wait<1>();
-  else cp_async_wait<2>();
-}
-
 // Descriptors of a 16-bit operand tile, 128-byte swizzle, eight-row groups 1024 bytes apart.  K-major:
 // a row's 64 elements are contiguous (the leading offset is not used).  MN-major (V of BF16 tiles, rows
 // are tokens): the leading offset leads to the next 64 channels.
@@ -212,13 +206,6 @@ __device__ __forceinline__ uint4 bf16x8_to_f16x8(const uint4& v, float f) {
 
 // -- producers -----------------------------------------------------------------------------------
 
-// Items of K/V work in order: K0, then K1 V0, K2 V1, ... and the last V: K runs a tile ahead of V, because an issuer
-// forms the next scores of its stream between the two halves of a tile's P V.
-struct Item { int t; bool is_v; };
-__device__ __forceinline__ Item item_of(int i, int items) {
-  if (i == items - 1) return {(items >> 1) - 1, true};
-  return (i & 1) ? Item{(i + 1) >> 1, false} : i == 0 ? Item{0, false} : Item{(i >> 1) - 1, true};
-}
 template <class SM>
 struct Producer {
   const ChunkAttention& a;
@@ -248,7 +235,6 @@ struct Producer {
       const bool ok = tok < valid;
       cp_async16(dst + swizzled(tok, unit), src + (ok ? tok : 0) * stride + unit * 8, ok);
     }
-    if (!is_v && warp == 0 && lane == 0) sm.tile_valid[(tile - w.begin) & 7] = valid;
   }
 
   // row warp * 32 + lane of a raw slot (the fetch's 64-byte swizzle undone), dequantised into an operand tile; a
@@ -282,91 +268,98 @@ struct Producer {
   }
 };
 
-// Page bytes, in the order of the items, up to RAW of them ahead of their expansion: one tensor copy of the head's
-// 128 x 64 bytes and one bulk copy of its scales each.  Page ids are fetched 32 at a time.
+// Page bytes into the raw slots, in the order K0 K1 V0 K2 V1 ... V(pages - 1): K a tile ahead of V, because an issuer
+// forms the next scores of its stream between the two halves of a tile's P V.  One tensor copy of the head's 128 x 64
+// bytes and one bulk copy of its scales each; page ids are fetched 32 at a time.
 template <class SM>
 __device__ __forceinline__ void fetch(const ChunkAttention& a, const ChunkMaps& maps, SM& sm, const Work& w, int row, int kvh,
                                       int lane) {
-  constexpr int RAW = SM::kRaw;
   constexpr uint32_t kAll = 0xffffffffu;
   const ChunkCache& c = a.c;
-  const int items = 2 * (w.end - w.begin), first_page = w.begin + w.bf16_tiles - w.fresh - w.tail_tiles;
-  const int32_t* table = c.page_table + (int64_t)row * c.page_table_row_stride + first_page;
-  const int pages = w.end - w.begin - w.bf16_tiles;
+  const int pages = w.end - w.begin - w.bf16_tiles, items = 2 * pages;
+  const int32_t* table = c.page_table + (int64_t)row * c.page_table_row_stride + w.begin + w.bf16_tiles - w.fresh - w.tail_tiles;
   int held[2] = {-1, -1}, ids[2] = {0, 0};       // K and V are a tile apart: 32 ids each
   int j = 0;
-  for (int item = 0; item < items; ++item) {
-    const Item n = item_of(item, items);
-    if (n.t < w.bf16_tiles) continue;
-    const int p = n.t - w.bf16_tiles, slot = j % RAW;
-    if (held[n.is_v] != p >> 5) {
-      held[n.is_v] = p >> 5;
+  for (; j < items; ++j) {
+    const bool is_v = j == items - 1 || (j > 0 && !(j & 1));
+    const int p = j == items - 1 ? pages - 1 : is_v ? (j >> 1) - 1 : (j + 1) >> 1;
+    const int ring = is_v ? SM::kRawV : SM::kRawK, turn = p / ring, slot = p - turn * ring + (is_v ? SM::kRawK : 0);
+    if (held[is_v] != p >> 5) {
+      held[is_v] = p >> 5;
       const int at = (p & ~31) + lane;
-      ids[n.is_v] = at < pages ? table[at] : -1;
+      ids[is_v] = at < pages ? table[at] : -1;
     }
-    const int64_t page = __shfl_sync(kAll, ids[n.is_v], p & 31);
+    const int64_t page = __shfl_sync(kAll, ids[is_v], p & 31);
     const bool ok = page >= 0 && page < c.num_pages;
-    if (j >= RAW && !__all_sync(kAll, mbar_wait(&sm.raw_empty[slot], (j / RAW - 1) & 1, sm, c.status))) break;
+    if (turn > 0 && !__all_sync(kAll, mbar_wait(&sm.raw_empty[slot], (turn - 1) & 1, sm, c.status))) break;
     if (lane == 0) {
-      if (!n.is_v) {
-        sm.tile_valid[n.t & 7] = ok ? 128 : 0;
+      if (!is_v) {
+        sm.page_ok[(w.bf16_tiles + p) & 7] = ok;
         if (!ok) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
       }
       if (ok) {
         mbar_expect_tx(&sm.raw_full[slot], kRawBytes);
         const uint32_t dst = smem_u32(sm.raw[slot]);
-        if (n.is_v) tma_load_4d(dst, &maps.v, &sm.raw_full[slot], 0, 0, kvh, (int)page);
+        if (is_v) tma_load_4d(dst, &maps.v, &sm.raw_full[slot], 0, 0, kvh, (int)page);
         else tma_load_4d(dst, &maps.k, &sm.raw_full[slot], 0, kvh, 0, (int)page);
-        bulk_load(dst + 8192, (n.is_v ? c.v_sf + page * c.v_sf_pitch : c.k_sf + page * c.k_sf_pitch) + kvh * kSfBlockBytes,
+        bulk_load(dst + 8192, (is_v ? c.v_sf + page * c.v_sf_pitch : c.k_sf + page * c.k_sf_pitch) + kvh * kSfBlockBytes,
                   kSfBlockBytes, &sm.raw_full[slot]);
       } else {
         mbar_arrive(&sm.raw_full[slot]);
       }
     }
     __syncwarp();
-    ++j;
   }
-  // nothing lands in shared memory after the CTA is gone, also after an expired wait
+  // nothing lands in shared memory after the CTA is gone, also after an expired wait: the last loads of each slot
   const unsigned long long t0 = global_ns();
-  for (int k = j > RAW ? j - RAW : 0; k < j; ++k)
-    while (!mbar_try(&sm.raw_full[k % RAW], (k / RAW) & 1) && global_ns() - t0 < 200000000ull) {}
+  const int fetched[2] = {j == 0 ? 0 : min((j >> 1) + 1, pages), j == items ? pages : j == 0 ? 0 : (j - 1) >> 1};
+  for (int v = 0; v < 2; ++v) {
+    const int ring = v ? SM::kRawV : SM::kRawK;
+    for (int p = max(0, fetched[v] - ring); p < fetched[v]; ++p)
+      while (!mbar_try(&sm.raw_full[p % ring + (v ? SM::kRawK : 0)], (p / ring) & 1) && global_ns() - t0 < 200000000ull) {}
+  }
 }
 
+// One warpgroup makes the K operands, one the V operands.
 template <class SM>
-__device__ __forceinline__ void produce(const ChunkAttention& a, SM& sm, const Work& w, int kvh, int warp, int lane) {
-  constexpr int RAW = SM::kRaw;
+__device__ __forceinline__ void produce(const ChunkAttention& a, SM& sm, const Work& w, int kvh, int warp, int lane, bool is_v) {
   Producer<SM> p{a, sm, w, kvh, warp, lane};
-  const int items = 2 * (w.end - w.begin);
-  auto empty = [&](const Item& n) -> bool {       // the operand stage of the tile before last has been used
-    return n.t < 2 || mbar_wait(n.is_v ? &sm.v_empty[n.t & 1] : &sm.k_empty[n.t & 1], ((n.t >> 1) - 1) & 1, sm, a.c.status);
+  uint8_t (*stage)[kOperandBytes] = is_v ? sm.v : sm.k;
+  uint64_t *full = is_v ? sm.v_full : sm.k_full, *empty = is_v ? sm.v_empty : sm.k_empty;
+  const int tiles = w.end - w.begin, last = is_v ? SM::kRaw : SM::kRawK;
+  int slot = is_v ? SM::kRawK : 0;
+  uint32_t parity = 0;
+  auto wait_empty = [&](int t) -> bool {       // the products of the tile before last are through
+    return t < 2 || mbar_wait(&empty[t & 1], ((t >> 1) - 1) & 1, sm, a.c.status);
   };
-  int next = 0, in_flight = 0, j = 0;     // first item not looked at, BF16 items issued and not landed, page items so far
-  for (int item = 0; item < items; ++item) {
-    // BF16 items go straight into an operand stage, two items ahead at most (the last V one: it follows its own K
-    // at two), once that stage is empty - what frees it must not wait for an item that is not through here yet.
-    // (Their last one is V of tile bf16_tiles - 1, item 2 * bf16_tiles at most.)
-    for (; next <= 2 * w.bf16_tiles && next < items && next <= item + (next == items - 1 ? 1 : 2); ++next) {
-      const Item n = item_of(next, items);
-      if (n.t >= w.bf16_tiles) continue;
-      if (!empty(n)) goto out;
-      p.issue_bf16(w.begin + n.t, n.is_v, smem_u32(n.is_v ? sm.v[n.t & 1] : sm.k[n.t & 1]));
-      cp_async_commit();
-      ++in_flight;
-    }
-    const Item n = item_of(item, items);
-    if (n.t < w.bf16_tiles) {
-      cp_async_wait_most(--in_flight);
-    } else {
-      const int slot = j % RAW;
-      if (!mbar_wait(&sm.raw_full[slot], (j / RAW) & 1, sm, a.c.status) || !empty(n)) goto out;
-      p.expand(sm.raw[slot], n.is_v ? sm.v[n.t & 1] : sm.k[n.t & 1], sm.tile_valid[n.t & 7] != 0);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.raw_empty[slot]);
-      ++j;
-    }
+  auto hand_over = [&](int t) {
     fence_proxy_async();
     __syncwarp();
-    if (lane == 0) mbar_arrive(n.is_v ? &sm.v_full[n.t & 1] : &sm.k_full[n.t & 1]);
+    if (lane == 0) mbar_arrive(&full[t & 1]);
+  };
+  // BF16 tiles: copied straight into an operand stage, the next one in flight while this one lands
+  for (int t = 0; t <= w.bf16_tiles; ++t) {
+    if (t < w.bf16_tiles) {
+      if (!__all_sync(0xffffffffu, wait_empty(t))) goto out;
+      p.issue_bf16(w.begin + t, is_v, smem_u32(stage[t & 1]));
+    }
+    cp_async_commit();
+    if (t > 0) {
+      cp_async_wait<1>();
+      __syncwarp();
+      hand_over(t - 1);
+    }
+  }
+  for (int t = w.bf16_tiles; t < tiles; ++t) {      // pages: through this operand's ring of raw slots
+    if (!__all_sync(0xffffffffu, mbar_wait(&sm.raw_full[slot], parity, sm, a.c.status) && wait_empty(t))) goto out;
+    p.expand(sm.raw[slot], stage[t & 1], sm.page_ok[t & 7] != 0);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.raw_empty[slot]);
+    hand_over(t);
+    if (++slot == last) {
+      slot = is_v ? SM::kRawK : 0;
+      parity ^= 1;
+    }
   }
 out:
   cp_async_wait<0>();
@@ -388,7 +381,7 @@ __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Wor
   const int tiles = w.end - w.begin;
   const uint64_t q_desc = desc_k_major(smem_u32(sm.q[SM::kQTiles > 1 ? qt : 0]));
   const uint32_t col_s = tmem + kColS + s * 128, col_o = tmem + kColO + s * 128;
-  bool f16_seen = w.bf16_tiles == 0;
+  bool ready = mbar_wait(&sm.q_ready[qt], 0, sm, status), f16_seen = w.bf16_tiles == 0;
   auto scores = [&](int t, int half) -> bool {
     const bool bf16 = t < w.bf16_tiles;
     if (half == 0) {
@@ -411,7 +404,8 @@ __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Wor
     if (half) commit(&sm.k_empty[t & 1], leader);
     return true;
   };
-  bool ok = first < tiles && scores(first, 0) && scores(first, 1);
+  ready = __all_sync(kAll, ready);
+  bool ok = ready && first < tiles && scores(first, 0) && scores(first, 1);
   for (int t = first, u = 0; t < tiles && ok; t += stride, ++u) {
     const bool bf16 = t < w.bf16_tiles;
     ok = mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, sm, status);
@@ -444,7 +438,7 @@ struct QueryRow {
   float shift;           // q . key_shift
 };
 
-__device__ __forceinline__ QueryRow query_row(const ChunkAttention& a, const Work& w, int kvh, int tile, int r) {
+__device__ __forceinline__ QueryRow query_row(const Work& w, int kvh, int tile, int r) {
   QueryRow q;
   const int in_tile = r / w.group;
   q.token = w.token0 + tile * w.tile_tokens + in_tile;
@@ -570,10 +564,16 @@ __device__ __forceinline__ void exp64(uint32_t* raw, uint64_t scale, uint64_t mi
 
 template <class SM>
 __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int stream, int r,
-                                        const QueryRow& q, RowState& state) {
+                                        int kvh, QueryRow& q, RowState& state) {
   uint32_t* status = a.c.status;
   constexpr uint32_t kAll = 0xffffffffu;
   const int qt = w.two ? stream : 0;
+  q = query_row(w, kvh, qt, r);
+  load_query(a, w, kvh, r, q, sm.q[SM::kQTiles > 1 ? qt : 0], w.two || stream == 0);
+  if (w.two || stream == 0) {
+    fence_proxy_async();
+    mbar_arrive(&sm.q_ready[qt]);
+  }
   const uint32_t lanes = (uint32_t)(r & ~31) << 16;
   const uint32_t col_s = tmem + lanes + kColS + stream * 128, col_o = tmem + lanes + kColO + stream * 128;
   const bool warp_live = __any_sync(kAll, q.live);
@@ -594,7 +594,7 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
       if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream][half], u & 1, sm, status))) return false;
       tc_fence_after();
       if (half == 0) {
-        limit = tile < w.fresh ? q.token - tile * 128 + 1 : sm.tile_valid[t & 7];
+        limit = tile < w.fresh ? q.token - tile * 128 + 1 : bf16 ? w.r.tail : sm.page_ok[t & 7] ? 128 : 0;
       } else {
         limit -= 64;
         if (t == w.bf16_tiles - 1 && w.bf16_tiles < w.end - w.begin) {
@@ -759,7 +759,7 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
   const int stream = warp >> 2, r = threadIdx.x & 127;
   if (w.begin == w.end) {      // nothing in this range of the keys
     if (stream < (w.two ? 2 : 1)) {
-      const QueryRow q = query_row(a, w, kvh, stream, r);
+      const QueryRow q = query_row(w, kvh, stream, r);
       if (q.live) a.lse_partial[((int64_t)split * a.c.tokens + w.r.first + q.token) * a.heads_q + q.head] = -INFINITY;
     }
     return;
@@ -775,6 +775,7 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
       mbar_init(&sm.p_ready[i][0], 128);
       mbar_init(&sm.p_ready[i][1], 128);
       mbar_init(&sm.o_done[i], 1);
+      mbar_init(&sm.q_ready[i], 128);
       mbar_init(&sm.q_f16[i], 128);
     }
     mbar_init(&sm.all_done, 2);
@@ -790,28 +791,22 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  QueryRow q{};
-  if (stream < 2) {
-    const int tile = w.two ? stream : 0;
-    q = query_row(a, w, kvh, tile, r);
-    load_query(a, w, kvh, r, q, sm.q[QTILES > 1 ? tile : 0], w.two || stream == 0);
-    fence_proxy_async();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  // registers: 512 threads at 128, shared out as 2 x 192 + 88 + 40 = 4 x 128
+  // registers: 640 threads at 96, shared out as 2 x 144 + 2 x 72 + 48 = 5 x 96
   if (stream < 2) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     RowState state{-INFINITY, 0.f};
-    const bool ok = softmax(a, sm, w, tmem, stream, r, q, state);
+    QueryRow q;
+    const bool ok = softmax(a, sm, w, tmem, stream, r, kvh, q, state);
     finish(a, sm, w, tmem, stream, r, q, state, split, ok);
-  } else if (stream == 2) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    produce(a, sm, w, kvh, warp - kProducerWarp0, lane);
+  } else if (stream < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    produce(a, sm, w, kvh, warp & 3, lane, stream == 3);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp < kIssueWarp + 2) {
       issue(a, sm, w, tmem, warp - kIssueWarp);
       // nothing of this CTA's is in flight when its tensor memory goes back, also after an expired wait
