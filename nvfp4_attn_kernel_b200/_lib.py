@@ -293,11 +293,12 @@ class ChunkArgs(ctypes.Structure):
 
 def _declare_chunk(lib) -> None:
     lib.nvfp4_chunk_attention.restype = c_int
-    lib.nvfp4_chunk_attention.argtypes = [ctypes.POINTER(ChunkArgs), c_void_p]
+    # the argument block as packed bytes, or byref(ChunkArgs)
+    lib.nvfp4_chunk_attention.argtypes = [c_void_p, c_void_p]
     lib.nvfp4_chunk_attention_workspace_bytes.restype = c_size_t
     lib.nvfp4_chunk_attention_workspace_bytes.argtypes = [c_int, c_int, c_int]
     lib.nvfp4_append_chunk.restype = c_int
-    lib.nvfp4_append_chunk.argtypes = [ctypes.POINTER(ChunkArgs), c_void_p]
+    lib.nvfp4_append_chunk.argtypes = [c_void_p, c_void_p]
     lib.nvfp4_dequantize_pages.restype = c_int
     lib.nvfp4_dequantize_pages.argtypes = [c_void_p, c_int64] * 4 + [c_int64, c_void_p, c_int, c_int, c_void_p,
                                                                      c_void_p, c_void_p, c_void_p]

@@ -13,6 +13,7 @@ A step that continues sequences is :func:`fp4_chunk_attention` in every layer, t
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
 
@@ -22,106 +23,111 @@ PAGE_SIZE = 128
 HEAD_DIM = 128
 
 
-def _device_of(tensor: torch.Tensor, name: str) -> torch.device:
-    if not tensor.is_cuda:
+_BF16, _I32 = torch.bfloat16, torch.int32
+# the argument block of the C ABI (struct nvfp4_chunk_args), packed in one call: filling a ctypes structure field by field
+# costs more than the checks
+_BLOCK = struct.Struct("@" + "Pq" * 4 + "qPqiPPPqPP" + "PPPqqPiiiiP" + "PqqPqPifiPN" + "PP")
+
+
+def _device_index(tensor: torch.Tensor, name: str) -> int:
+    index = tensor.get_device()
+    if index < 0:
         raise ValueError(f"{name} must be a CUDA tensor")
-    return tensor.device
+    return index
 
 
-def _tokens(tensor: torch.Tensor, name: str, device: torch.device) -> tuple[int, int]:
-    """Rows and heads of a BF16 [tokens, heads, 128] tensor that is dense within a token."""
-    shape, stride = tensor.shape, tensor.stride()
-    if tensor.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != HEAD_DIM or tensor.device != device:
-        raise ValueError(f"{name} must be BF16 [tokens, heads, 128] on {device}")
-    if stride[2] != 1 or (shape[1] > 1 and stride[1] != HEAD_DIM):
+def _tokens(tensor: torch.Tensor, name: str, index: int) -> tuple[int, int, int]:
+    """Rows, heads and token stride of a BF16 [tokens, heads, 128] tensor that is dense within a token."""
+    if tensor.dtype is not _BF16 or tensor.ndim != 3 or tensor.get_device() != index:
+        raise ValueError(f"{name} must be BF16 [tokens, heads, 128] on device {index}")
+    tokens, heads, dim = tensor.shape
+    token_stride, head_stride, unit = tensor.stride()
+    if dim != HEAD_DIM:
+        raise ValueError(f"{name} must be BF16 [tokens, heads, 128] on device {index}")
+    if unit != 1 or (head_stride != HEAD_DIM and heads > 1):
         raise ValueError(f"{name} must be dense within a token")
-    return shape[0], shape[1]
+    return tokens, heads, token_stride if tokens > 1 else heads * HEAD_DIM
 
 
-def _index(tensor: torch.Tensor, name: str, length: int, device: torch.device) -> int:
-    if tensor.dtype is not torch.int32 or tensor.device != device or tensor.shape != (length,) or \
-            (length > 1 and tensor.stride(0) != 1):
-        raise ValueError(f"{name} must be contiguous INT32 of shape [{length}] on {device}")
+def _index(tensor: torch.Tensor, name: str, length: int, index: int) -> int:
+    """Address of a contiguous INT32 vector."""
+    if tensor.dtype is not _I32 or tensor.get_device() != index or tensor.ndim != 1 or tensor.shape[0] != length or \
+            not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous INT32 of shape [{length}] on device {index}")
     return tensor.data_ptr()
 
 
-def _page_regions(args, key_pages_fp4, key_scales, value_pages_fp4, value_scales, device) -> int:
-    """Check the four page regions and enter them in an argument block; returns the KV head count."""
-    if key_pages_fp4.ndim != 4:
+def _page_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, index):
+    """Check the four page regions; their addresses and pitches, the page and the KV head count."""
+    shape = key_pages_fp4.shape
+    if len(shape) != 4 or shape[1] != PAGE_SIZE or shape[3] != HEAD_DIM // 2:
         raise ValueError("key_pages_fp4 must be packed FP4 with shape [pages, 128, heads_kv, 64]")
-    pages, page, heads, half = key_pages_fp4.shape
-    if page != PAGE_SIZE or half != HEAD_DIM // 2:
-        raise ValueError("key_pages_fp4 must be packed FP4 with shape [pages, 128, heads_kv, 64]")
-    want_scales = (pages, 32, 4, 1, 4, 2, heads)
-    for name, tensor, shape, inner in (
-        ("key_pages_fp4", key_pages_fp4, None, (heads * 64, 64, 1)),
-        ("value_pages_fp4", value_pages_fp4, (pages, heads, HEAD_DIM, 64), (HEAD_DIM * 64, 64, 1)),
-        ("key_scales", key_scales, want_scales, (16, 4, 1024, 1, 512, 1024)),
-        ("value_scales", value_scales, want_scales, (16, 4, 1024, 1, 512, 1024)),
-    ):
-        if tensor.device != device or tensor.element_size() != 1:
-            raise ValueError(f"{name} must hold bytes on {device}")
-        if shape is not None and tensor.shape != shape:
-            raise ValueError(f"{name} must have shape {shape}")
-        if tensor.stride()[1:] != inner:
-            raise ValueError(f"{name} must be dense within a page, in the quantisers' layout")
-    args.k_packed, args.k_pitch = key_pages_fp4.data_ptr(), key_pages_fp4.stride(0)
-    args.k_sf, args.k_sf_pitch = key_scales.data_ptr(), key_scales.stride(0)
-    args.v_packed, args.v_pitch = value_pages_fp4.data_ptr(), value_pages_fp4.stride(0)
-    args.v_sf, args.v_sf_pitch = value_scales.data_ptr(), value_scales.stride(0)
-    args.num_pages, args.heads_kv = pages, heads
-    return heads
+    pages, _, heads, _ = shape
+    if value_pages_fp4.shape != (pages, heads, HEAD_DIM, 64):
+        raise ValueError(f"value_pages_fp4 must have shape {(pages, heads, HEAD_DIM, 64)}")
+    want = (pages, 32, 4, 1, 4, 2, heads)
+    if key_scales.shape != want or value_scales.shape != want:
+        raise ValueError(f"key_scales and value_scales must have shape {want}")
+    k, ks, v, vs = key_pages_fp4.stride(), key_scales.stride(), value_pages_fp4.stride(), value_scales.stride()
+    if k[1:] != (heads * 64, 64, 1) or v[1:] != (HEAD_DIM * 64, 64, 1):
+        raise ValueError("key_pages_fp4 and value_pages_fp4 must be dense within a page")
+    if ks[1:] != (16, 4, 1024, 1, 512, 1024) or vs[1:] != (16, 4, 1024, 1, 512, 1024):
+        raise ValueError("key_scales and value_scales must use the quantisers' layout")
+    for tensor in (key_pages_fp4, key_scales, value_pages_fp4, value_scales):
+        if tensor.get_device() != index or tensor.element_size() != 1:
+            raise ValueError(f"the page regions must hold bytes on device {index}")
+    return (key_pages_fp4.data_ptr(), k[0], key_scales.data_ptr(), ks[0], value_pages_fp4.data_ptr(), v[0],
+            value_scales.data_ptr(), vs[0]), pages, heads
 
 
-def _fill(key, value, key_pages_fp4, key_scales, value_pages_fp4, value_scales, fp4_page_table, seqused_fp4,
-          chunk_start_loc, max_chunk_len, residual, key_shift, status, device):
-    """The argument block with everything the attention and the append share, checked."""
-    args = _lib.ChunkArgs()
-    heads = _page_regions(args, key_pages_fp4, key_scales, value_pages_fp4, value_scales, device)
-    tokens, key_heads = _tokens(key, "key", device)
-    if (tokens, key_heads) != _tokens(value, "value", device) or key_heads != heads:
+def _shared(key, value, key_pages_fp4, key_scales, value_pages_fp4, value_scales, fp4_page_table, seqused_fp4,
+            chunk_start_loc, max_chunk_len, residual, key_shift, status, index):
+    """What the attention and the append share, checked: the first fields of the argument block, and rows, tokens,
+    the chunk bound, KV heads, table columns, pages."""
+    regions, pages, heads = _page_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, index)
+    tokens, key_heads, key_stride = _tokens(key, "key", index)
+    value_tokens, value_heads, value_stride = _tokens(value, "value", index)
+    if tokens != value_tokens or key_heads != heads or value_heads != heads:
         raise ValueError("key and value must have the same tokens, and the pages' heads")
-    args.key, args.value = key.data_ptr(), value.data_ptr()
-    width = heads * HEAD_DIM
-    args.key_token_stride = key.stride(0) if tokens > 1 else width
-    args.value_token_stride = value.stride(0) if tokens > 1 else width
-    if fp4_page_table.dtype is not torch.int32 or fp4_page_table.ndim != 2 or fp4_page_table.device != device or \
-            (fp4_page_table.shape[1] > 1 and fp4_page_table.stride(1) != 1):
-        raise ValueError(f"fp4_page_table must be INT32 [rows, max_pages] on {device}, dense within a row")
+    if fp4_page_table.dtype is not _I32 or fp4_page_table.ndim != 2 or fp4_page_table.get_device() != index:
+        raise ValueError(f"fp4_page_table must be INT32 [rows, max_pages] on device {index}")
     rows, columns = fp4_page_table.shape
-    args.page_table, args.max_pages = fp4_page_table.data_ptr(), columns
-    args.page_table_row_stride = fp4_page_table.stride(0) if rows > 1 else columns
-    args.seqused_fp4 = _index(seqused_fp4, "seqused_fp4", rows, device)
-    args.chunk_start = _index(chunk_start_loc, "chunk_start_loc", rows + 1, device)
-    if not isinstance(max_chunk_len, int) or max_chunk_len < 0:
+    row_stride, unit = fp4_page_table.stride()
+    if unit != 1 and columns > 1:
+        raise ValueError("fp4_page_table must be dense within a row")
+    if type(max_chunk_len) is not int or max_chunk_len < 0:
         raise ValueError(f"max_chunk_len must be a non-negative int, got {max_chunk_len!r}")
-    args.rows, args.tokens, args.max_chunk = rows, tokens, min(max_chunk_len, tokens)
     tail_key, tail_value, tail_ids, tail_used = residual
-    if any(item is not None for item in residual):
-        if any(item is None for item in residual):
+    if tail_key is None and tail_value is None and tail_ids is None and tail_used is None:
+        tail = (0, 0, 0, 0, 0)
+    else:
+        if tail_key is None or tail_value is None or tail_ids is None or tail_used is None:
             raise ValueError("the four residual arguments must be provided together")
-        for name, tensor in (("residual_key_pages_bf16", tail_key), ("residual_value_pages_bf16", tail_value)):
-            if tensor.dtype is not torch.bfloat16 or tensor.device != device or tensor.ndim != 4 or \
-                    tensor.shape[1:] != (PAGE_SIZE, heads, HEAD_DIM) or not tensor.is_contiguous():
-                raise ValueError(f"{name} must be contiguous BF16 [pages, 128, {heads}, 128] on {device}")
-        if tail_key.shape[0] != tail_value.shape[0]:
-            raise ValueError("the residual caches must have the same pages")
-        args.tail_key, args.tail_value, args.tail_pages = tail_key.data_ptr(), tail_value.data_ptr(), tail_key.shape[0]
-        args.tail_ids = _index(tail_ids, "residual_page_ids", rows, device)
-        args.seqused_tail = _index(tail_used, "seqused_residual", rows, device)
+        shape = tail_key.shape
+        for tensor in (tail_key, tail_value):
+            if tensor.dtype is not _BF16 or tensor.get_device() != index or tensor.shape != shape or len(shape) != 4 or \
+                    shape[1] != PAGE_SIZE or shape[2] != heads or shape[3] != HEAD_DIM or not tensor.is_contiguous():
+                raise ValueError("residual_key_pages_bf16 and residual_value_pages_bf16 must be contiguous BF16 "
+                                 f"[pages, 128, {heads}, 128] on device {index}")
+        tail = (tail_key.data_ptr(), tail_value.data_ptr(), shape[0], _index(tail_ids, "residual_page_ids", rows, index),
+                _index(tail_used, "seqused_residual", rows, index))
+    shift = 0
     if key_shift is not None:
-        if key_shift.dtype is not torch.bfloat16 or key_shift.device != device or \
-                key_shift.shape != (heads, HEAD_DIM) or not key_shift.is_contiguous():
-            raise ValueError(f"key_shift must be contiguous BF16 [{heads}, 128] on {device}")
-        args.key_shift = key_shift.data_ptr()
-    if status is not None:
-        args.status = _status(status, device)
-    return args
+        if key_shift.dtype is not _BF16 or key_shift.get_device() != index or key_shift.shape != (heads, HEAD_DIM) or \
+                not key_shift.is_contiguous():
+            raise ValueError(f"key_shift must be contiguous BF16 [{heads}, 128] on device {index}")
+        shift = key_shift.data_ptr()
+    chunk = max_chunk_len if max_chunk_len < tokens else tokens
+    fields = (*regions, pages, fp4_page_table.data_ptr(), row_stride if rows > 1 else columns, columns,
+              _index(seqused_fp4, "seqused_fp4", rows, index), *tail,
+              _index(chunk_start_loc, "chunk_start_loc", rows + 1, index), key.data_ptr(), value.data_ptr(), key_stride,
+              value_stride, shift, rows, tokens, chunk, heads, 0 if status is None else _status(status, index))
+    return fields, rows, tokens, chunk, heads, columns, pages
 
 
-def _status(status: torch.Tensor, device: torch.device) -> int:
-    if status.element_size() != 4 or status.is_floating_point() or status.numel() < 1 or status.device != device:
-        raise ValueError(f"status must be one 32-bit integer on {device}")
+def _status(status: torch.Tensor, index: int) -> int:
+    if status.element_size() != 4 or status.is_floating_point() or status.numel() < 1 or status.get_device() != index:
+        raise ValueError(f"status must be one 32-bit integer on device {index}")
     return status.data_ptr()
 
 
@@ -165,8 +171,30 @@ def _check_metadata(table, seqused_fp4, starts, max_chunk_len, tokens, residual,
 
 def chunk_split_heuristic(rows: int, tokens: int, max_chunk_len: int, heads_q: int, heads_kv: int, max_pages: int, *,
                           sms: int) -> int:
-    """Ranges that each row's keys are cut into."""
-    return 1
+    """Ranges that each row's keys are cut into, by predicted makespan.
+
+    A CTA takes one KV head of one row and a block of query rows (one tile of 128 query rows, two where a chunk has
+    more), one CTA per SM.  It costs about 8 us before and after its K/V tiles and 1.4 us a tile with one query tile, 2.4
+    with two (measured: 32 rows x 4 tokens after 4096 tokens 107 us in two waves of 33 tiles, 512 tokens after 16384
+    332 us); a split adds a launch of 4 us and its partial results' way through memory.  The table's width stands for
+    the lengths, which the host does not know.  Only counts that just fill a number of waves are tried; one that is
+    not a twentieth faster than whole rows is not taken.
+    """
+    if rows < 1 or tokens < 1 or max_chunk_len < 1 or sms < 1:
+        return 1
+    tile = 128 // (heads_q // heads_kv)
+    per, tile_us = (tile, 1.4) if max_chunk_len <= tile else (2 * tile, 2.4)
+    ctas = min(rows * -(-max_chunk_len // per), tokens // per + rows) * heads_kv
+    tiles = max_pages + -(-max_chunk_len // 128)
+    best, best_us = 1, 0.95 * -(-ctas // sms) * (8.0 + tiles * tile_us)
+    partial_us = tokens * heads_q * 1032 / 5e6
+    for waves in (1, 2, 3, 5, 7):
+        splits = min(waves * sms // ctas, 32, tiles)
+        if splits > best:
+            us = -(-ctas * splits // sms) * (8.0 + -(-tiles // splits) * tile_us) + 4.0 + splits * partial_us
+            if us < best_us:
+                best, best_us = splits, us
+    return best
 
 
 def fp4_chunk_attention(
@@ -219,56 +247,54 @@ def fp4_chunk_attention(
     are the lengths before it.  Unlike ``fp4_decode`` the query and the probabilities are not quantised.
     Returns ``out[:tokens]``, or a fresh tensor whose padding rows are undefined.
     """
-    device = _device_of(query, "query")
-    args = _fill(key, value, key_pages_fp4, key_scales, value_pages_fp4, value_scales, fp4_page_table, seqused_fp4,
-                 chunk_start_loc, max_chunk_len,
-                 (residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, seqused_residual), key_shift,
-                 status, device)
-    shape, stride = query.shape, query.stride()
-    if query.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1:
+    index = _device_index(query, "query")
+    residual = (residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, seqused_residual)
+    fields, rows, tokens, chunk, heads, columns, pages = _shared(
+        key, value, key_pages_fp4, key_scales, value_pages_fp4, value_scales, fp4_page_table, seqused_fp4,
+        chunk_start_loc, max_chunk_len, residual, key_shift, status, index)
+    if query.dtype is not _BF16 or query.ndim != 3 or query.shape[2] != HEAD_DIM or query.stride(2) != 1:
         raise ValueError("query must be BF16 [tokens, heads_q, 128] with unit channel stride")
-    tokens, heads_q = shape[0], shape[1]
-    if tokens != args.tokens:
-        raise ValueError(f"query has {tokens} tokens, key and value have {args.tokens}")
-    args.query, args.heads_q = query.data_ptr(), heads_q
-    args.q_token_stride = stride[0] if tokens > 1 else heads_q * HEAD_DIM
-    args.q_head_stride = stride[1] if heads_q > 1 else HEAD_DIM
+    query_tokens, heads_q, _ = query.shape
+    token_stride, head_stride, _ = query.stride()
+    if query_tokens != tokens:
+        raise ValueError(f"query has {query_tokens} tokens, key and value have {tokens}")
     if out is None:
-        out = torch.empty(tokens, heads_q, HEAD_DIM, dtype=torch.bfloat16, device=device)
+        out = torch.empty(tokens, heads_q, HEAD_DIM, dtype=_BF16, device=query.device)
+        out_tokens, out_stride = tokens, heads_q * HEAD_DIM
     else:
-        out_tokens, out_heads = _tokens(out, "out", device)
+        out_tokens, out_heads, out_stride = _tokens(out, "out", index)
         if out_heads != heads_q or out_tokens < tokens:
             raise ValueError(f"out must have shape [at least {tokens}, {heads_q}, 128]")
-    args.out, args.out_token_stride = out.data_ptr(), out.stride(0) if out.shape[0] > 1 else heads_q * HEAD_DIM
+    lse_address = 0
     if lse is not None:
-        if lse.dtype is not torch.float32 or lse.device != device or lse.ndim != 2 or lse.shape[0] < tokens or \
+        if lse.dtype is not torch.float32 or lse.get_device() != index or lse.ndim != 2 or lse.shape[0] < tokens or \
                 lse.shape[1] != heads_q or not lse.is_contiguous():
-            raise ValueError(f"lse must be contiguous FP32 of shape [at least {tokens}, {heads_q}] on {device}")
-        args.lse = lse.data_ptr()
+            raise ValueError(f"lse must be contiguous FP32 of shape [at least {tokens}, {heads_q}] on device {index}")
+        lse_address = lse.data_ptr()
     scale = HEAD_DIM ** -0.5 if softmax_scale is None else softmax_scale
-    if not math.isfinite(scale) or scale <= 0.0:
+    if not 0.0 < scale < math.inf:
         raise ValueError("softmax_scale must be finite and positive")
-    args.softmax_scale = scale
     if num_splits is None:
-        num_splits = chunk_split_heuristic(args.rows, tokens, args.max_chunk, heads_q, args.heads_kv, args.max_pages,
-                                           sms=_sm_count(device))
-    elif not isinstance(num_splits, int) or not 1 <= num_splits <= 128:
+        num_splits = chunk_split_heuristic(rows, tokens, chunk, heads_q, heads, columns, sms=_sm_count(index)) \
+            if heads_q >= heads else 1
+    elif type(num_splits) is not int or not 1 <= num_splits <= 128:
         raise ValueError(f"num_splits must be 1 to 128, got {num_splits!r}")
-    args.num_splits = num_splits
-    need = chunk_workspace_bytes(tokens, heads_q, num_splits)
-    if need:
+    space, need = 0, 0
+    if num_splits > 1:
+        need = chunk_workspace_bytes(tokens, heads_q, num_splits)
         if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        elif workspace.dtype is not torch.uint8 or workspace.device != device or not workspace.is_contiguous() or \
+            workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+        elif workspace.dtype is not torch.uint8 or workspace.get_device() != index or not workspace.is_contiguous() or \
                 workspace.numel() < need:
-            raise ValueError(f"workspace must be contiguous UINT8 of at least {need} bytes on {device}")
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
+            raise ValueError(f"workspace must be contiguous UINT8 of at least {need} bytes on device {index}")
+        space = workspace.data_ptr()
     if not trusted_metadata:
-        _check_metadata(fp4_page_table, seqused_fp4, chunk_start_loc, max_chunk_len, tokens,
-                        (residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, seqused_residual),
-                        args.num_pages, False)
-    _launch("nvfp4_chunk_attention", args, device)
-    return out[:tokens] if out.shape[0] != tokens else out
+        _check_metadata(fp4_page_table, seqused_fp4, chunk_start_loc, max_chunk_len, tokens, residual, pages, False)
+    block = _BLOCK.pack(*fields, query.data_ptr(), token_stride if tokens > 1 else heads_q * HEAD_DIM,
+                        head_stride if heads_q > 1 else HEAD_DIM, out.data_ptr(), out_stride, lse_address, heads_q, scale,
+                        num_splits, space, need, 0, 0)
+    _launch(_lib.load().nvfp4_chunk_attention, index, block)
+    return out if out_tokens == tokens else out[:tokens]
 
 
 def append_kv_chunk(
@@ -304,23 +330,22 @@ def append_kv_chunk(
     A row whose metadata is out of range, or whose table has no column left, keeps its cache and lengths and is
     flagged in ``status``; with ``trusted_metadata=False`` such a batch is refused before anything is written.
     """
-    device = _device_of(key, "key")
+    index = _device_index(key, "key")
     residual = (residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, seqused_residual)
-    if any(item is None for item in residual):
+    if residual_key_pages_bf16 is None:
         raise ValueError("append_kv_chunk needs the four residual arguments")
-    args = _fill(key, value, key_pages_fp4, key_scales, value_pages_fp4, value_scales, fp4_page_table, seqused_fp4,
-                 chunk_start_loc, max_chunk_len, residual, key_shift, status, device)
-    rows = args.rows
+    fields, rows, tokens, _, _, _, pages = _shared(
+        key, value, key_pages_fp4, key_scales, value_pages_fp4, value_scales, fp4_page_table, seqused_fp4,
+        chunk_start_loc, max_chunk_len, residual, key_shift, status, index)
     if seqused_fp4_out is None or seqused_residual_out is None:
-        fresh = torch.empty(2, rows, dtype=torch.int32, device=device)
-        seqused_fp4_out = fresh[0] if seqused_fp4_out is None else seqused_fp4_out
-        seqused_residual_out = fresh[1] if seqused_residual_out is None else seqused_residual_out
-    args.seqused_fp4_out = _index(seqused_fp4_out, "seqused_fp4_out", rows, device)
-    args.seqused_tail_out = _index(seqused_residual_out, "seqused_residual_out", rows, device)
+        full, rest = torch.empty(2, rows, dtype=_I32, device=key.device).unbind()
+        seqused_fp4_out = full if seqused_fp4_out is None else seqused_fp4_out
+        seqused_residual_out = rest if seqused_residual_out is None else seqused_residual_out
+    after = (_index(seqused_fp4_out, "seqused_fp4_out", rows, index),
+             _index(seqused_residual_out, "seqused_residual_out", rows, index))
     if not trusted_metadata:
-        _check_metadata(fp4_page_table, seqused_fp4, chunk_start_loc, max_chunk_len, args.tokens, residual,
-                        args.num_pages, True)
-    _launch("nvfp4_append_chunk", args, device)
+        _check_metadata(fp4_page_table, seqused_fp4, chunk_start_loc, max_chunk_len, tokens, residual, pages, True)
+    _launch(_lib.load().nvfp4_append_chunk, index, _BLOCK.pack(*fields, 0, 0, 0, 0, 0, 0, 0, 0.0, 0, 0, 0, *after))
     return seqused_fp4_out, seqused_residual_out
 
 
@@ -338,34 +363,26 @@ def dequantize_pages(
     """Pages back to BF16: K and V ``[len(page_ids), 128, heads_kv, 128]``, exact (``e2m1 * e4m3`` has at most six
     significant bits).  Keys come back as they are cached, shifted ones shifted.  An id outside the cache gives
     zeros and sets a bit of ``status``.  One launch."""
-    device = _device_of(key_pages_fp4, "key_pages_fp4")
-    args = _lib.ChunkArgs()
-    heads = _page_regions(args, key_pages_fp4, key_scales, value_pages_fp4, value_scales, device)
+    index = _device_index(key_pages_fp4, "key_pages_fp4")
+    regions, pages, heads = _page_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, index)
     if page_ids.ndim != 1:
         raise ValueError("page_ids must be contiguous 1-D INT32")
     count = page_ids.shape[0]
-    ids = _index(page_ids, "page_ids", count, device)
+    ids = _index(page_ids, "page_ids", count, index)
     shape = (count, PAGE_SIZE, heads, HEAD_DIM)
-    outs = []
-    for name, tensor in (("key_out", key_out), ("value_out", value_out)):
-        if tensor is None:
-            tensor = torch.empty(shape, dtype=torch.bfloat16, device=device)
-        elif tensor.dtype is not torch.bfloat16 or tensor.device != device or tensor.shape != shape or \
-                not tensor.is_contiguous():
-            raise ValueError(f"{name} must be contiguous BF16 {shape} on {device}")
-        outs.append(tensor)
-    flag = None if status is None else _status(status, device)
-    call = _lib.load().nvfp4_dequantize_pages
-    index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    block = (args.k_packed, args.k_pitch, args.k_sf, args.k_sf_pitch, args.v_packed, args.v_pitch, args.v_sf,
-             args.v_sf_pitch, args.num_pages, ids, count, heads, outs[0].data_ptr(), outs[1].data_ptr(), flag, stream)
-    if torch.cuda.current_device() == index:
-        _lib.check(call(*block))
-    else:
-        with torch.cuda.device(index):
-            _lib.check(call(*block))
-    return outs[0], outs[1]
+    if key_out is None:
+        key_out = torch.empty(shape, dtype=_BF16, device=page_ids.device)
+    elif key_out.dtype is not _BF16 or key_out.get_device() != index or key_out.shape != shape or \
+            not key_out.is_contiguous():
+        raise ValueError(f"key_out must be contiguous BF16 {shape} on device {index}")
+    if value_out is None:
+        value_out = torch.empty(shape, dtype=_BF16, device=page_ids.device)
+    elif value_out.dtype is not _BF16 or value_out.get_device() != index or value_out.shape != shape or \
+            not value_out.is_contiguous():
+        raise ValueError(f"value_out must be contiguous BF16 {shape} on device {index}")
+    _launch(_lib.load().nvfp4_dequantize_pages, index, *regions, pages, ids, count, heads, key_out.data_ptr(),
+            value_out.data_ptr(), None if status is None else _status(status, index))
+    return key_out, value_out
 
 
 def chunk_workspace_bytes(tokens: int, heads_q: int, num_splits: int) -> int:
@@ -377,19 +394,19 @@ def chunk_workspace_bytes(tokens: int, heads_q: int, num_splits: int) -> int:
 _SM_COUNT: dict[int, int] = {}
 
 
-def _sm_count(device: torch.device) -> int:
-    count = _SM_COUNT.get(device.index)
+def _sm_count(index: int) -> int:
+    count = _SM_COUNT.get(index)
     if count is None:
-        count = _SM_COUNT[device.index] = torch.cuda.get_device_properties(device).multi_processor_count
+        count = _SM_COUNT[index] = torch.cuda.get_device_properties(index).multi_processor_count
     return count
 
 
-def _launch(name: str, args, device: torch.device) -> None:
-    call = getattr(_lib.load(), name)
-    index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
+def _launch(call, index: int, *arguments) -> None:
+    """A call of the library on the current stream of device ``index``."""
     if torch.cuda.current_device() == index:
-        _lib.check(call(args, stream))
+        code = call(*arguments, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            _lib.check(call(args, stream))
+            code = call(*arguments, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        _lib.check(code)

@@ -55,7 +55,8 @@ class PagePool:
                         tail.shape[2] != PAGE_SIZE or tail.shape[4] != 128 or not tail.is_contiguous() or \
                         tail.shape != tail_key.shape:
                     raise ValueError(f"{name} must be contiguous BF16 [layers, slots, 128, heads_kv, 128] on {device}")
-        self.blocks, self.device = blocks, device
+        self.blocks, self.device, self._index = blocks, device, device.index
+        self._lib = _lib.load()
         self.num_pages, self.block_bytes = int(shape[0]), int(shape[1])
         self.reserved_pages = reserved_pages
         self.refs = torch.zeros(self.num_pages, dtype=torch.int32, device=device) if refs is None else refs
@@ -63,36 +64,41 @@ class PagePool:
         self.tail_key, self.tail_value = tail_key, tail_value
         self.status = torch.zeros(1, dtype=torch.int32, device=device) if status is None else status
         self._vector(self.status, "status", 1)
+        self._fork_tail = (None, None, 0, 0, 0, 0, 1) if tail_key is None else (
+            tail_key.data_ptr(), tail_value.data_ptr(), tail_key.stride(0), tail_key.stride(1), tail_key.shape[0],
+            tail_key.shape[1], tail_key.shape[3])
         self._bases = torch.tensor([b.data_ptr() for b in blocks], dtype=torch.int64, device=device)
         self._scratch = torch.empty(3 * self.num_pages + 1, dtype=torch.int32, device=device)
-        if self._scratch.numel() * 4 < _lib.load().nvfp4_pool_compact_workspace_bytes(self.num_pages):
+        if self._scratch.numel() * 4 < self._lib.nvfp4_pool_compact_workspace_bytes(self.num_pages):
             raise RuntimeError("the pool's scratch does not match the library's")
 
     # -- checks ------------------------------------------------------------------------------
 
     def _vector(self, tensor: torch.Tensor, name: str, length: int | None = None) -> int:
-        if tensor.dtype is not torch.int32 or tensor.ndim != 1 or tensor.device != self.device or \
+        if tensor.dtype is not torch.int32 or tensor.ndim != 1 or tensor.get_device() != self._index or \
                 not tensor.is_contiguous() or (length is not None and tensor.shape[0] != length):
             want = "n" if length is None else length
             raise ValueError(f"{name} must be contiguous INT32 [{want}] on {self.device}")
         return tensor.data_ptr()
 
     def _table(self, page_table: torch.Tensor, pages_held: torch.Tensor) -> tuple[int, int, int, int, int]:
-        if page_table.dtype is not torch.int32 or page_table.ndim != 2 or page_table.device != self.device or \
-                (page_table.shape[1] > 1 and page_table.stride(1) != 1) or page_table.stride(0) < page_table.shape[1]:
+        if page_table.dtype is not torch.int32 or page_table.ndim != 2 or page_table.get_device() != self._index:
             raise ValueError(f"page_table must be INT32 [rows, columns] on {self.device}, dense within a row")
         rows, columns = page_table.shape
-        return page_table.data_ptr(), page_table.stride(0), columns, rows, self._vector(pages_held, "pages_held", rows)
+        row_stride, unit = page_table.stride()
+        if (unit != 1 and columns > 1) or (row_stride < columns and rows > 1):
+            raise ValueError(f"page_table must be INT32 [rows, columns] on {self.device}, dense within a row")
+        return page_table.data_ptr(), row_stride, columns, rows, self._vector(pages_held, "pages_held", rows)
 
-    def _call(self, name: str, *args) -> None:
-        call = getattr(_lib.load(), name)
-        index = self.device.index
-        stream = torch._C._cuda_getCurrentRawStream(index)
+    def _call(self, call, *args) -> None:
+        index = self._index
         if torch.cuda.current_device() == index:
-            _lib.check(call(*args, stream))
+            code = call(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
             with torch.cuda.device(index):
-                _lib.check(call(*args, stream))
+                code = call(*args, torch._C._cuda_getCurrentRawStream(index))
+        if code:
+            _lib.check(code)
 
     # -- operations --------------------------------------------------------------------------
 
@@ -100,7 +106,7 @@ class PagePool:
         """Give back what the rows of the list (INT32) hold; ``pages_held`` of them becomes 0.  A row named twice is
         released once; that, a row that does not exist and a page nobody holds set bits of ``status``."""
         table, stride, columns, count, held = self._table(page_table, pages_held)
-        self._call("nvfp4_pool_release", self._vector(rows, "rows"), rows.shape[0], table, stride, columns, count, held,
+        self._call(self._lib.nvfp4_pool_release, self._vector(rows, "rows"), rows.shape[0], table, stride, columns, count, held,
                    self.refs.data_ptr(), self.num_pages, self.status.data_ptr())
 
     def fork(self, sources: torch.Tensor, targets: torch.Tensor, page_table: torch.Tensor, pages_held: torch.Tensor,
@@ -113,19 +119,15 @@ class PagePool:
         table, stride, columns, count, held = self._table(page_table, pages_held)
         if sources.shape != targets.shape:
             raise ValueError("sources and targets must have the same length")
-        tail = (None, None, 0, 0, 0, 0, 1)
         slots = None
         if self.tail_key is not None:
             if row_to_slot is None:
                 raise ValueError("a pool with tails needs row_to_slot to fork")
-            layers, slot_count, _, heads, _ = self.tail_key.shape
-            tail = (self.tail_key.data_ptr(), self.tail_value.data_ptr(), self.tail_key.stride(0),
-                    self.tail_key.stride(1), layers, slot_count, heads)
             slots = self._vector(row_to_slot, "row_to_slot", count)
-        self._call("nvfp4_pool_fork", self._vector(sources, "sources"), self._vector(targets, "targets"),
+        self._call(self._lib.nvfp4_pool_fork, self._vector(sources, "sources"), self._vector(targets, "targets"),
                    sources.shape[0], table, stride, columns, count, held, self._vector(seqused_fp4, "seqused_fp4", count),
                    self._vector(seqused_residual, "seqused_residual", count), slots, self.refs.data_ptr(),
-                   self.num_pages, *tail, self.status.data_ptr())
+                   self.num_pages, *self._fork_tail, self.status.data_ptr())
 
     def compact(self, page_table: torch.Tensor, pages_held: torch.Tensor) -> torch.Tensor:
         """Move the live pages into the lowest ids, in every layer: with L of them, the k-th at or above L goes to the
@@ -134,7 +136,7 @@ class PagePool:
         one given."""
         table, stride, columns, count, held = self._table(page_table, pages_held)
         live = torch.empty(1, dtype=torch.int32, device=self.device)
-        self._call("nvfp4_pool_compact", self._bases.data_ptr(), len(self.blocks), self.block_bytes, self.num_pages,
+        self._call(self._lib.nvfp4_pool_compact, self._bases.data_ptr(), len(self.blocks), self.block_bytes, self.num_pages,
                    self.reserved_pages, self.refs.data_ptr(), table, stride, columns, count, held,
                    self._scratch.data_ptr(), self._scratch.numel() * 4, live.data_ptr(), self.status.data_ptr())
         return live
@@ -155,13 +157,13 @@ class PagePool:
                 raise ValueError(f"page ids must be below {self.num_pages}")
             if len(set(written)) != len(written) or set(written) & {s for s, _ in pairs}:
                 raise ValueError("a page may be copied to once, and not from a page that is copied to")
-        self._call("nvfp4_pool_copy", self._bases.data_ptr(), len(self.blocks), self.block_bytes, self.num_pages, src,
+        self._call(self._lib.nvfp4_pool_copy, self._bases.data_ptr(), len(self.blocks), self.block_bytes, self.num_pages, src,
                    dst, source_pages.shape[0], self.status.data_ptr())
 
     def free_list(self) -> tuple[torch.Tensor, torch.Tensor]:
         """The free pages, ascending, then -1 (INT32 ``[pages]``), and how many they are (INT32 ``[1]``)."""
         ids = torch.empty(self.num_pages, dtype=torch.int32, device=self.device)
         count = torch.empty(1, dtype=torch.int32, device=self.device)
-        self._call("nvfp4_pool_free_list", self.refs.data_ptr(), self.num_pages, self.reserved_pages, ids.data_ptr(),
+        self._call(self._lib.nvfp4_pool_free_list, self.refs.data_ptr(), self.num_pages, self.reserved_pages, ids.data_ptr(),
                    count.data_ptr())
         return ids, count

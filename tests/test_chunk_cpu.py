@@ -19,6 +19,15 @@ def test_struct_mirror_matches_header_field_order():
     assert re.findall(r"\b([a-z_0-9]+)\s*;", body) == [name for name, _ in L.ChunkArgs._fields_]
 
 
+def test_packed_block_is_the_struct():
+    from nvfp4_attn_kernel_b200.nvfp4_decode_kernel.chunk import _BLOCK
+
+    assert _BLOCK.size == ctypes.sizeof(L.ChunkArgs)
+    values = [i + 0.5 if kind is ctypes.c_float else i + 1 for i, (_, kind) in enumerate(L.ChunkArgs._fields_)]
+    args = L.ChunkArgs.from_buffer_copy(_BLOCK.pack(*values))
+    assert [getattr(args, name) for name, _ in L.ChunkArgs._fields_] == values
+
+
 def test_workspace_sizes():
     from nvfp4_attn_kernel_b200.nvfp4_decode_kernel.chunk import chunk_workspace_bytes
 
@@ -58,7 +67,7 @@ def arguments(**changes):
     (dict(num_pages=-1), "page counts"),
 ])
 def test_shared_refusals(entry, changes, words):
-    assert getattr(L.load(), entry)(arguments(**changes), None) == L.ERR_INVALID
+    assert getattr(L.load(), entry)(ctypes.byref(arguments(**changes)), None) == L.ERR_INVALID
     assert words in L.last_error()
 
 
@@ -71,11 +80,11 @@ def test_attention_refusals():
                            (dict(out=SOME + 8), "alignment"), (dict(q_head_stride=129), "alignment"),
                            (dict(out_token_stride=128), "dense in a token"), (dict(num_splits=2), "workspace"),
                            (dict(num_splits=2, workspace=SOME, workspace_bytes=2 * 5 * 8 * 516 - 1), "workspace")):
-        assert call(arguments(**changes), None) == L.ERR_INVALID
+        assert call(ctypes.byref(arguments(**changes)), None) == L.ERR_INVALID
         assert words in L.last_error()
-    assert call(arguments(heads_q=18), None) == L.ERR_UNSUPPORTED
+    assert call(ctypes.byref(arguments(heads_q=18)), None) == L.ERR_UNSUPPORTED
     for empty in (dict(rows=0), dict(tokens=0), dict(max_chunk=0)):
-        assert call(arguments(**empty), None) == 0
+        assert call(ctypes.byref(arguments(**empty)), None) == 0
 
 
 def test_append_refusals():
@@ -83,9 +92,9 @@ def test_append_refusals():
     assert call(None, None) == L.ERR_INVALID
     for changes, words in ((dict(tail_key=None, tail_value=None, tail_ids=None, seqused_tail=None), "needs the BF16 tail"),
                            (dict(seqused_fp4_out=None), "need buffers"), (dict(seqused_tail_out=SOME + 32), "of their own")):
-        assert call(arguments(**changes), None) == L.ERR_INVALID
+        assert call(ctypes.byref(arguments(**changes)), None) == L.ERR_INVALID
         assert words in L.last_error()
-    assert call(arguments(rows=0), None) == 0
+    assert call(ctypes.byref(arguments(rows=0)), None) == 0
 
 
 def test_dequantize_refusals():
