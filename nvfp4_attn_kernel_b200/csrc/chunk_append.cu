@@ -6,6 +6,8 @@
 // of one page column of one row, K or V, so nothing is shared between CTAs but the tail page: the
 // first page is sealed from the old tail while the leftover overwrites it.  Both are therefore
 // done by the same CTA, reads first, whenever both happen; else the leftover has a CTA of its own.
+#include <cuda_fp16.h>
+
 #include "chunk_common.cuh"
 
 namespace nvfp4 {
@@ -21,52 +23,60 @@ struct AppendSmem {
   __align__(16) uint8_t scales[kSfBlockBytes];
 };
 
-// Channels [g*16, g*16 + 16) of stream token p of this head: from the tail below t, else from the
-// chunk, shifted.
-__device__ __forceinline__ void load_group(const ChunkCache& c, const ChunkRow& r, int head, bool is_value, int p, int g,
-                                           uint4& a, uint4& b) {
+// Channels [g*16, g*16 + 16) of stream token p of this head: from the tail below t, else from the chunk.
+__device__ __forceinline__ const uint4* group_at(const ChunkCache& c, const ChunkRow& r, int head, bool is_value, int p, int g) {
   const uint16_t* src;
   if (p < r.tail) {
-    src = (is_value ? c.tail_value : c.tail_key) +
-          (((int64_t)r.tail_id * kPage + p) * c.heads_kv + head) * kHeadDim + g * 16;
-    a = *reinterpret_cast<const uint4*>(src);
-    b = *reinterpret_cast<const uint4*>(src + 8);
-    return;
+    src = (is_value ? c.tail_value : c.tail_key) + ((int64_t)r.tail_id * kPage + p) * c.heads_kv * kHeadDim;
+  } else {
+    const int64_t token = (int64_t)r.first + (p - r.tail);
+    src = is_value ? c.value + token * c.value_stride : c.key + token * c.key_stride;
   }
-  const int64_t token = (int64_t)r.first + (p - r.tail);
-  src = (is_value ? c.value + token * c.value_stride : c.key + token * c.key_stride) + head * kHeadDim + g * 16;
-  a = *reinterpret_cast<const uint4*>(src);
-  b = *reinterpret_cast<const uint4*>(src + 8);
-  if (!is_value && c.key_shift) {
-    const uint16_t* m = c.key_shift + head * kHeadDim + g * 16;
-    float x[16], y[16];
-    unpack_bf16x8(a, x);
-    unpack_bf16x8(b, x + 8);
-    unpack_bf16x8(*reinterpret_cast<const uint4*>(m), y);
-    unpack_bf16x8(*reinterpret_cast<const uint4*>(m + 8), y + 8);
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {   // one BF16 subtract per channel, as the page quantiser's shift
-      const __nv_bfloat162 d = __floats2bfloat162_rn(x[2 * i] - y[2 * i], x[2 * i + 1] - y[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&d);
-    }
-    a = make_uint4(w[0], w[1], w[2], w[3]);
-    b = make_uint4(w[4], w[5], w[6], w[7]);
-  }
+  return reinterpret_cast<const uint4*>(src + head * kHeadDim + g * 16);
 }
+
+// The key shift's 16 channels of a group, as fp32.
+__device__ __forceinline__ void load_shift(const ChunkCache& c, int head, int g, float (&m)[16]) {
+  const uint4* at = reinterpret_cast<const uint4*>(c.key_shift + head * kHeadDim + g * 16);
+  unpack_bf16x8(at[0], m);
+  unpack_bf16x8(at[1], m + 8);
+}
+
+__device__ __forceinline__ uint4 pack_bf16x8(const float* x) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 d = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&d);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+constexpr int kItems = kPage * 8 / kAppendThreads;   // groups of a page and head per thread
 
 __device__ __forceinline__ void seal_key(const ChunkCache& c, const ChunkRow& r, AppendSmem& sm, int head, int column,
                                          int64_t page) {
   uint8_t* packed = c.k_packed + page * c.k_pitch;
+  const int g = threadIdx.x & 7, tok0 = threadIdx.x >> 3;     // a thread keeps its group of channels
+  uint4 a[kItems], b[kItems];
 #pragma unroll
-  for (int k = 0; k < kPage * 8 / kAppendThreads; ++k) {
-    const int it = threadIdx.x + k * kAppendThreads;
-    const int tok = it >> 3, g = it & 7;
-    uint4 a, b;
-    load_group(c, r, head, false, column * kPage + tok, g, a, b);
+  for (int k = 0; k < kItems; ++k) {      // every load of the thread first: the kernel lives on loads in flight
+    const uint4* at = group_at(c, r, head, false, column * kPage + tok0 + k * (kAppendThreads / 8), g);
+    a[k] = at[0];
+    b[k] = at[1];
+  }
+  float shift[16];
+  if (c.key_shift) load_shift(c, head, g, shift);
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int tok = tok0 + k * (kAppendThreads / 8);
     float x[16];
-    unpack_bf16x8(a, x);
-    unpack_bf16x8(b, x + 8);
+    unpack_bf16x8(a[k], x);
+    unpack_bf16x8(b[k], x + 8);
+    if (c.key_shift && column * kPage + tok >= r.tail) {      // one BF16 subtract per channel; the tail's are shifted
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __bfloat162float(__float2bfloat16_rn(x[i] - shift[i]));
+    }
     uint32_t lo, hi;
     uint8_t s;
     quantize_group16(x, lo, hi, s);
@@ -81,19 +91,25 @@ __device__ __forceinline__ void seal_key(const ChunkCache& c, const ChunkRow& r,
 
 __device__ __forceinline__ void seal_value(const ChunkCache& c, const ChunkRow& r, AppendSmem& sm, int head, int column,
                                            int64_t page) {
+  {
+    const int g = threadIdx.x & 7, tok0 = threadIdx.x >> 3;
+    uint4 a[kItems], b[kItems];
 #pragma unroll
-  for (int k = 0; k < kPage * 8 / kAppendThreads; ++k) {
-    const int it = threadIdx.x + k * kAppendThreads;
-    const int tok = it >> 3, g = it & 7;
-    uint4 a, b;
-    load_group(c, r, head, true, column * kPage + tok, g, a, b);
-    uint32_t* dst = sm.tile + tok * kTileWords + g * 8;
-    dst[0] = a.x; dst[1] = a.y; dst[2] = a.z; dst[3] = a.w;
-    dst[4] = b.x; dst[5] = b.y; dst[6] = b.z; dst[7] = b.w;
+    for (int k = 0; k < kItems; ++k) {
+      const uint4* at = group_at(c, r, head, true, column * kPage + tok0 + k * (kAppendThreads / 8), g);
+      a[k] = at[0];
+      b[k] = at[1];
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      uint32_t* dst = sm.tile + (tok0 + k * (kAppendThreads / 8)) * kTileWords + g * 8;
+      dst[0] = a[k].x; dst[1] = a[k].y; dst[2] = a[k].z; dst[3] = a[k].w;
+      dst[4] = b[k].x; dst[5] = b[k].y; dst[6] = b[k].z; dst[7] = b[k].w;
+    }
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kHeadDim * 8 / kAppendThreads; ++k) {
+  for (int k = 0; k < kItems; ++k) {
     const int it = threadIdx.x + k * kAppendThreads;
     const int g = it >> 7, d = it & 127;
     float x[16];
@@ -158,84 +174,123 @@ append_chunk_kernel(const ChunkCache c, int32_t* seqused_fp4_out, int32_t* sequs
   uint16_t* tail = (is_value ? c.tail_value : c.tail_key) + ((int64_t)r.tail_id * kPage * c.heads_kv + head) * kHeadDim;
   for (int it = threadIdx.x; it < (rest - begin) * 8; it += kAppendThreads) {
     const int p = begin + (it >> 3), g = it & 7;
-    uint4 a, b;
-    load_group(c, r, head, is_value, sealed * kPage + p, g, a, b);
+    const uint4* at = group_at(c, r, head, is_value, sealed * kPage + p, g);
+    uint4 a = at[0], b = at[1];
+    if (!is_value && c.key_shift) {      // (the leftover is the chunk's: what the tail keeps stays where it is)
+      float x[16], m[16];
+      unpack_bf16x8(a, x);
+      unpack_bf16x8(b, x + 8);
+      load_shift(c, head, g, m);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] -= m[i];
+      a = pack_bf16x8(x);
+      b = pack_bf16x8(x + 8);
+    }
     uint16_t* dst = tail + (int64_t)p * c.heads_kv * kHeadDim + g * 16;
     *reinterpret_cast<uint4*>(dst) = a;
     *reinterpret_cast<uint4*>(dst + 8) = b;
   }
 }
 
-// 16 nibbles of one group times its scale, as BF16 (exact: at most six significant bits).
-__device__ __forceinline__ void dequantize_group(uint2 nibbles, uint8_t scale, float (&x)[16]) {
-  const float s = e4m3_to_f32(scale);
+// Eight nibbles times their scale (an FP16 pair of it) as BF16 pairs, in order: exact, since the product has at most
+// six significant bits, which both formats hold.
+__device__ __forceinline__ uint4 dequantize8(uint32_t nibbles, uint32_t scale2) {
+  uint32_t h[4], r[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(nibbles));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = e2m1_to_f32(nibbles.x >> (4 * i)) * s;
-    x[8 + i] = e2m1_to_f32(nibbles.y >> (4 * i)) * s;
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), *reinterpret_cast<const __half2*>(&scale2));
+    const float2 f = __half22float2(v);
+    const __nv_bfloat162 o = __floats2bfloat162_rn(f.x, f.y);
+    r[i] = *reinterpret_cast<const uint32_t*>(&o);
   }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ uint32_t scale_pair(uint8_t e4m3) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(e4m3 * 0x0101)));
+  return h;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
+constexpr int kOutWords = 68;   // a token's 64 channel pairs and four words of padding: 16-byte rows
+// Word of channel pair `pair` of a token in the V tile.  Eight more words per 32 tokens: a warp stores eight pairs of
+// four tokens that are 32 apart, each lane then in a bank of its own.
+__device__ __forceinline__ int out_word(int tok, int pair) { return tok * kOutWords + (tok >> 5) * 8 + pair; }
 
-// grid (pages, heads_kv * 2)
+// grid (pages, heads_kv * 2).  K rows are rows of the result: four bytes in, sixteen out per thread.  V is packed along the
+// tokens: a thread takes 32 tokens of two neighbouring channels, and the page is turned in shared memory.  Bound by
+// memory: 144 bytes in and 512 out per token and head.
 __global__ void __launch_bounds__(kAppendThreads)
 dequantize_pages_kernel(const ChunkCache c, const int32_t* __restrict__ page_ids, uint16_t* __restrict__ key_out,
                         uint16_t* __restrict__ value_out) {
-  __shared__ uint32_t tile[kPage * kTileWords];
+  __shared__ __align__(16) uint32_t tile[kPage * kOutWords + 3 * 8];
   const int item = blockIdx.x;
   const bool is_value = (int)blockIdx.y >= c.heads_kv;
   const int head = is_value ? blockIdx.y - c.heads_kv : blockIdx.y;
   const int64_t page = page_ids[item];
   const bool valid = page >= 0 && page < c.num_pages;
   if (!valid && blockIdx.y == 0 && threadIdx.x == 0) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
-  const int64_t first = (int64_t)item * kPage;
-  uint16_t* out = (is_value ? value_out : key_out) + (first * c.heads_kv + head) * kHeadDim;
+  uint16_t* out = (is_value ? value_out : key_out) + ((int64_t)item * kPage * c.heads_kv + head) * kHeadDim;
   const int64_t pitch = (int64_t)c.heads_kv * kHeadDim;
+  const int part = threadIdx.x & 15;      // of a row of the result: eight channels
+  if (!valid) {
+    for (int tok = threadIdx.x >> 4; tok < kPage; tok += kAppendThreads / 16)
+      *reinterpret_cast<uint4*>(out + tok * pitch + part * 8) = make_uint4(0, 0, 0, 0);
+    return;
+  }
   if (!is_value) {
+    const uint8_t* packed = c.k_packed + page * c.k_pitch + head * 64 + part * 4;
+    const uint8_t* scales = c.k_sf + page * c.k_sf_pitch + head * kSfBlockBytes;
+    uint32_t n[8];
+    uint8_t s[8];
 #pragma unroll
-    for (int k = 0; k < kPage * 8 / kAppendThreads; ++k) {
-      const int it = threadIdx.x + k * kAppendThreads;
-      const int tok = it >> 3, g = it & 7;
-      uint4 a = make_uint4(0, 0, 0, 0), b = a;
-      if (valid) {
-        const uint2 n = *reinterpret_cast<const uint2*>(c.k_packed + page * c.k_pitch +
-                                                        ((int64_t)tok * c.heads_kv + head) * 64 + g * 8);
-        float x[16];
-        dequantize_group(n, c.k_sf[page * c.k_sf_pitch + head * kSfBlockBytes + sf_offset(tok, g)], x);
-        a = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-        b = make_uint4(pack_bf16(x[8], x[9]), pack_bf16(x[10], x[11]), pack_bf16(x[12], x[13]), pack_bf16(x[14], x[15]));
-      }
-      uint16_t* dst = out + tok * pitch + g * 16;
-      *reinterpret_cast<uint4*>(dst) = a;
-      *reinterpret_cast<uint4*>(dst + 8) = b;
+    for (int k = 0; k < 8; ++k) {
+      const int tok = (threadIdx.x >> 4) + k * (kAppendThreads / 16);
+      n[k] = __ldg(reinterpret_cast<const uint32_t*>(packed + (int64_t)tok * c.heads_kv * 64));
+      s[k] = __ldg(scales + sf_offset(tok, part >> 1));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int tok = (threadIdx.x >> 4) + k * (kAppendThreads / 16);
+      *reinterpret_cast<uint4*>(out + tok * pitch + part * 8) = dequantize8(n[k], scale_pair(s[k]));
     }
     return;
   }
-  if (valid) {
-    uint16_t* half = reinterpret_cast<uint16_t*>(tile);
+  {
+    const int piece = threadIdx.x & 3, pair = threadIdx.x >> 2;       // tokens 32 * piece ..., channels 2 * pair and the next
+    const uint8_t* packed = c.v_packed + page * c.v_pitch + ((int64_t)head * kHeadDim + 2 * pair) * 64 + piece * 16;
+    const uint8_t* scales = c.v_sf + page * c.v_sf_pitch + head * kSfBlockBytes;
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(packed)), b = __ldg(reinterpret_cast<const uint4*>(packed + 64));
+    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int k = 0; k < kHeadDim * 8 / kAppendThreads; ++k) {
-      const int it = threadIdx.x + k * kAppendThreads;
-      const int g = it >> 7, d = it & 127;
-      const uint2 n = *reinterpret_cast<const uint2*>(c.v_packed + page * c.v_pitch +
-                                                      ((int64_t)head * kHeadDim + d) * 64 + g * 8);
-      float x[16];
-      dequantize_group(n, c.v_sf[page * c.v_sf_pitch + head * kSfBlockBytes + sf_offset(d, g)], x);
+    for (int g = 0; g < 2; ++g) {
+      const uint32_t sa = scale_pair(__ldg(scales + sf_offset(2 * pair, 2 * piece + g)));
+      const uint32_t sb = scale_pair(__ldg(scales + sf_offset(2 * pair + 1, 2 * piece + g)));
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        half[(g * 16 + i) * (2 * kTileWords) + d] = (uint16_t)(__float_as_uint(x[i]) >> 16);   // exact in BF16
+      for (int half = 0; half < 2; ++half) {
+        const uint4 x = dequantize8(wa[2 * g + half], sa), y = dequantize8(wb[2 * g + half], sb);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        const int tok = piece * 32 + g * 16 + half * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          tile[out_word(tok + 2 * i, pair)] = __byte_perm(xs[i], ys[i], 0x5410);
+          tile[out_word(tok + 2 * i + 1, pair)] = __byte_perm(xs[i], ys[i], 0x7632);
+        }
+      }
     }
   }
   __syncthreads();
-  for (int it = threadIdx.x; it < kPage * 16; it += kAppendThreads) {
-    const int tok = it >> 4, q = it & 15;
-    const uint32_t* src = tile + tok * kTileWords + q * 4;
-    *reinterpret_cast<uint4*>(out + tok * pitch + q * 8) =
-        valid ? make_uint4(src[0], src[1], src[2], src[3]) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int tok = (threadIdx.x >> 4) + k * (kAppendThreads / 16);
+    *reinterpret_cast<uint4*>(out + tok * pitch + part * 8) = *reinterpret_cast<const uint4*>(tile + out_word(tok, part * 4));
   }
 }
 
