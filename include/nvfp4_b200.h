@@ -529,7 +529,8 @@ int nvfp4_decode_host_io(const nvfp4_decode_args* args, const void* q_host, size
  * max_chunk of them.  Its history is seqused_fp4[r] tokens in sealed NVFP4 pages (a multiple of 128)
  * followed by seqused_tail[r] tokens (0 to 128) in BF16 tail page tail_ids[r].  All of these live on
  * the device and nothing is read back; what is out of range is clamped, flagged in `status` and never
- * made an address.  Buffers behind the last row's tokens are not touched.
+ * made an address.  Buffers behind the last row's tokens are not touched.  At most 65535 rows, and
+ * 4194304 tokens of one row.
  */
 typedef struct nvfp4_chunk_args {
   /* NVFP4 pages, as in nvfp4_decode_args */

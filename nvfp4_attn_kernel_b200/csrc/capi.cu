@@ -743,23 +743,24 @@ size_t nvfp4_push_merge_inbox_floats(int world, int rows, int heads_q) {
 
 namespace {
 
-// The checks that the chunk entry points share; `tail` 0: must be absent or whole, 1: required.
+// The checks that the chunk entry points share.  (Buffers of a call without rows may be null, as an empty tensor's.)
 int chunk_cache(const nvfp4_chunk_args* a, const char* who, bool need_tail, nvfp4::ChunkCache* c) {
   if (!a) return fail(NVFP4_ERR_INVALID, "%s: null argument block", who);
   if (a->rows < 0 || a->tokens < 0 || a->max_chunk < 0) return fail(NVFP4_ERR_INVALID, "%s: negative extent", who);
   if (a->rows > 65535) return fail(NVFP4_ERR_INVALID, "%s: too many rows: %d", who, a->rows);
+  if (a->max_chunk > (1 << 22)) return fail(NVFP4_ERR_INVALID, "%s: max_chunk too large: %d", who, a->max_chunk);
   if (a->heads_kv < 1 || a->heads_kv > 128)
     return fail(NVFP4_ERR_INVALID, "%s: heads_kv out of range: %d", who, a->heads_kv);
   if (a->max_pages < 0 || a->num_pages < 0 || a->num_pages > INT32_MAX)
     return fail(NVFP4_ERR_INVALID, "%s: page counts out of range", who);
-  if (!a->seqused_fp4 || !a->chunk_start) return fail(NVFP4_ERR_INVALID, "%s: null lengths", who);
+  if (a->rows > 0 && (!a->seqused_fp4 || !a->chunk_start)) return fail(NVFP4_ERR_INVALID, "%s: null lengths", who);
   if (a->tokens > 0 && (!a->key || !a->value)) return fail(NVFP4_ERR_INVALID, "%s: key and value must be non-null", who);
   const int64_t width = (int64_t)a->heads_kv * 128;
   if (a->key_token_stride < width || a->value_token_stride < width || (a->key_token_stride % 8) ||
       (a->value_token_stride % 8) || !aligned16(a->key) || !aligned16(a->value) || !aligned16(a->key_shift))
     return fail(NVFP4_ERR_INVALID, "%s: key and value must be dense within a token and 16-byte aligned", who);
-  if (a->max_pages > 0) {
-    if (!a->page_table || !a->k_packed || !a->k_sf || !a->v_packed || !a->v_sf)
+  if (a->rows > 0 && a->max_pages > 0) {
+    if (!a->page_table || (a->num_pages > 0 && (!a->k_packed || !a->k_sf || !a->v_packed || !a->v_sf)))
       return fail(NVFP4_ERR_INVALID, "%s: page regions and table must be non-null", who);
     if (a->page_table_row_stride < a->max_pages)
       return fail(NVFP4_ERR_INVALID, "%s: page_table_row_stride is smaller than max_pages", who);
@@ -770,8 +771,8 @@ int chunk_cache(const nvfp4_chunk_args* a, const char* who, bool need_tail, nvfp
       return fail(NVFP4_ERR_INVALID, "%s: page regions need a page's bytes as pitch and 16-byte alignment", who);
   }
   const int given = !!a->tail_key + !!a->tail_value + !!a->tail_ids + !!a->seqused_tail;
-  if (given != 0 && given != 4) return fail(NVFP4_ERR_INVALID, "%s: the tail's four arguments go together", who);
-  if (need_tail && given == 0) return fail(NVFP4_ERR_INVALID, "%s: needs the BF16 tail", who);
+  if (a->rows > 0 && given != 0 && given != 4) return fail(NVFP4_ERR_INVALID, "%s: the tail's four arguments go together", who);
+  if (a->rows > 0 && need_tail && given == 0) return fail(NVFP4_ERR_INVALID, "%s: needs the BF16 tail", who);
   if (given && (!aligned16(a->tail_key) || !aligned16(a->tail_value) || a->tail_pages < 0))
     return fail(NVFP4_ERR_INVALID, "%s: tail pages must be 16-byte aligned", who);
   *c = nvfp4::ChunkCache{};
@@ -842,7 +843,6 @@ int nvfp4_append_chunk(const nvfp4_chunk_args* a, void* stream) {
   if (a->seqused_fp4_out == a->seqused_fp4 || a->seqused_tail_out == a->seqused_tail ||
       a->seqused_fp4_out == a->seqused_tail || a->seqused_tail_out == a->seqused_fp4)
     return fail(NVFP4_ERR_INVALID, "append_chunk: the lengths afterwards need buffers of their own");
-  if (a->max_chunk / 128 + 2 > 65535) return fail(NVFP4_ERR_INVALID, "append_chunk: max_chunk too large");
   cudaError_t e = nvfp4::launch_append_chunk(c, a->seqused_fp4_out, a->seqused_tail_out,
                                              static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "append_chunk launch");

@@ -4,10 +4,12 @@
 // tokens 0..i.  The G query heads of a KV head and the tokens of a chunk are packed into tiles of
 // 128 query rows, so a K/V tile that has been read (and dequantised) once serves all of them.  A CTA
 // takes one KV head of one row and two streams of work, S = Q K^T and O += P V on the tensor cores
-// (tcgen05, kind::f16, fp32 accumulators in tensor memory), a softmax warpgroup each:
+// (tcgen05, kind::f16, fp32 accumulators in tensor memory: 512 columns, all of them), a softmax warpgroup each:
 //   - two tiles of query rows over the same K/V tiles, when the chunk has more than one, or
 //   - one tile of query rows whose K/V tiles the streams take in turns, joined at the end.
-// While one stream computes its softmax the tensor cores work for the other.
+// While one stream computes its softmax the tensor cores work for the other.  Beside the two softmax warpgroups one
+// makes K operands and one V operands (dequantising pages that a warp of their own fetches with tensor copies, or
+// copying BF16 rows), a warp per stream issues the products.  Waits are bounded; an expired one sets a status bit.
 //
 // Operands.  A page's e2m1 * e4m3 is exact in FP16 (six significant bits, 2^-10 to 2688), and FP16
 // probabilities carry eleven bits, so pages meet an FP16 query: rounding a BF16 query row to FP16 loses
@@ -18,7 +20,13 @@
 //
 // Softmax.  A thread owns a query row: running maximum and sum in fp32, exponentials of the scaled
 // scores relative to a maximum that is only replaced when a new one exceeds it by 2^8 (O and the sum are
-// rescaled then; probabilities up to 2^8 fit both formats with the same relative precision).
+// rescaled then; probabilities up to 2^8 fit both formats with the same relative precision).  A chunk token whose
+// value is not finite makes earlier tokens of its 128-token tile not finite too (0 * inf in the product).
+//
+// What bounds it: long chunks, the softmax warpgroups (exponentials: 2048 of about 4600 clocks per pair of tiles, which
+// the two streams spend side by side; with the softmax left out the same products run at 1430 TFLOP/s).  1152 tokens of
+// 32 / 8 heads over 16384 tokens: 335 us = 954 TFLOP/s, 0.58 of a large library product's burst rate.  Short chunks, the
+// 128-row products and the operands' making: 32 rows x 4 tokens over 4096 tokens: 103 us for 160 MB.
 #include <cuda_fp16.h>
 
 #include "chunk_common.cuh"
@@ -40,6 +48,18 @@ constexpr float kRescaleLog2 = 8.f;
 constexpr uint32_t kColS = 0, kColO = 256;     // tensor-memory columns of stream 0; stream 1: + 128
 constexpr float kLn2 = 0.6931471805599453f;
 
+// What a CTA works on.
+struct Work {
+  ChunkRow r;
+  int group, tile_tokens;      // query heads per KV head; tokens in a tile of query rows
+  int token0;                  // first chunk token of tile 0
+  bool two;                    // two tiles of query rows; else one, the streams taking turns
+  int fresh, tail_tiles;       // K/V tiles: the chunk's, then the tail's (0 or 1), then the pages
+  int begin, end;              // this split's range of them
+  int bf16_tiles;              // of these, how many are BF16
+  int steps;                   // softmax steps of both streams together
+};
+
 // QTILES query tiles in shared memory, RAW slots of page bytes in flight, RAWK of them for K.  (A ring per operand: a
 // waiter on a slot's barrier has to have seen each of its phases, and loads do not land in the order of their issue.)
 template <int QTILES, int RAW>
@@ -56,6 +76,7 @@ struct ChunkSmem {
   int page_ok[8];            // whether page tile t was fetched (0: a refused id), at t % 8: the fetch is at most six
                              // tiles ahead of the softmax
   uint32_t tmem_base;
+  Work work;
   volatile int abort_flag;
 };
 
@@ -87,30 +108,21 @@ __device__ __forceinline__ uint32_t idesc(bool bf16, bool b_mn_major, uint32_t n
   return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// Issued by the lane whose `leader` is set, out of a warp that runs converged.
-__device__ __forceinline__ uint32_t elect_one() {
+__device__ __forceinline__ bool elect_one() {
   uint32_t leader;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
-  return leader;
+  return leader != 0;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate, uint32_t leader) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id),
-      "r"(accumulate), "r"(leader)
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate, uint32_t leader) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id),
-      "r"(accumulate), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leader)
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
       : "memory");
 }
 
@@ -171,18 +183,6 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 
 // Tensor maps of the packed page regions.
 struct ChunkMaps { CUtensorMap k, v; };
-
-// What a CTA works on.
-struct Work {
-  ChunkRow r;
-  int group, tile_tokens;      // query heads per KV head; tokens in a tile of query rows
-  int token0;                  // first chunk token of tile 0
-  bool two;                    // two tiles of query rows; else one, the streams taking turns
-  int fresh, tail_tiles;       // K/V tiles: the chunk's, then the tail's (0 or 1), then the pages
-  int begin, end;              // this split's range of them
-  int bf16_tiles;              // of these, how many are BF16
-  int steps;                   // softmax steps of both streams together
-};
 
 __device__ __forceinline__ int stream_steps(const Work& w, int stream) {
   return w.two ? w.end - w.begin : (w.end - w.begin + 1 - stream) >> 1;
@@ -278,18 +278,23 @@ __device__ __forceinline__ void fetch(const ChunkAttention& a, const ChunkMaps& 
   const ChunkCache& c = a.c;
   const int pages = w.end - w.begin - w.bf16_tiles, items = 2 * pages;
   const int32_t* table = c.page_table + (int64_t)row * c.page_table_row_stride + w.begin + w.bf16_tiles - w.fresh - w.tail_tiles;
-  int held[2] = {-1, -1}, ids[2] = {0, 0};       // K and V are a tile apart: 32 ids each
+  int held_k = -1, held_v = -1, ids_k = 0, ids_v = 0;       // K and V are a tile apart: 32 ids each
   int j = 0;
   for (; j < items; ++j) {
     const bool is_v = j == items - 1 || (j > 0 && !(j & 1));
     const int p = j == items - 1 ? pages - 1 : is_v ? (j >> 1) - 1 : (j + 1) >> 1;
     const int ring = is_v ? SM::kRawV : SM::kRawK, turn = p / ring, slot = p - turn * ring + (is_v ? SM::kRawK : 0);
-    if (held[is_v] != p >> 5) {
-      held[is_v] = p >> 5;
-      const int at = (p & ~31) + lane;
-      ids[is_v] = at < pages ? table[at] : -1;
+    if ((is_v ? held_v : held_k) != p >> 5) {
+      const int at = (p & ~31) + lane, id = at < pages ? table[at] : -1;
+      if (is_v) {
+        held_v = p >> 5;
+        ids_v = id;
+      } else {
+        held_k = p >> 5;
+        ids_k = id;
+      }
     }
-    const int64_t page = __shfl_sync(kAll, ids[is_v], p & 31);
+    const int64_t page = __shfl_sync(kAll, is_v ? ids_v : ids_k, p & 31);
     const bool ok = page >= 0 && page < c.num_pages;
     if (turn > 0 && !__all_sync(kAll, mbar_wait(&sm.raw_empty[slot], (turn - 1) & 1, sm, c.status))) break;
     if (lane == 0) {
@@ -369,21 +374,27 @@ out:
 
 // One warp per stream.  A tile's 128 tokens go through tensor memory as two halves of 64 columns: scores of a
 // half, its probabilities over the same columns, P V, scores of the next tile's half - so that the softmax
-// always has one half to work on while the tensor cores turn the other around (the products of one thread
-// complete in order).  The whole warp runs the loop, so addresses and descriptors stay in uniform registers; one
-// elected lane issues.
+// always has one half to work on while the tensor cores turn the other around.  (The scores of the next tile may
+// follow P V unawaited: the tensor core works off one thread's products in the order of their issue.)  With one issuer
+// for both streams the products alone ran at 650 TFLOP/s, with two at 1430: issuing an instruction costs its thread
+// about as long as the instruction runs.
 template <class SM>
-__device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int s) {
+__device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Work& work, uint32_t tensor_memory, int stream) {
   constexpr uint32_t kAll = 0xffffffffu;
   uint32_t* status = a.c.status;
-  const uint32_t leader = elect_one();
-  const int qt = w.two ? s : 0, first = w.two ? 0 : s, stride = w.two ? 1 : 2;
-  const int tiles = w.end - w.begin;
+  const bool leader = elect_one();
+  // (a value out of lane 0 is known to be the same in every lane, so that what follows from it can stay in uniform
+  // registers, where the tensor instructions take their operands from)
+  auto uniform = [](int v) { return __shfl_sync(kAll, v, 0); };
+  const int s = uniform(stream), bf16_tiles = uniform(work.bf16_tiles), tiles = uniform(work.end - work.begin);
+  const bool two = uniform(work.two);
+  const uint32_t tmem = uniform((int)tensor_memory);
+  const int qt = two ? s : 0, first = two ? 0 : s, stride = two ? 1 : 2;
   const uint64_t q_desc = desc_k_major(smem_u32(sm.q[SM::kQTiles > 1 ? qt : 0]));
   const uint32_t col_s = tmem + kColS + s * 128, col_o = tmem + kColO + s * 128;
-  bool ready = mbar_wait(&sm.q_ready[qt], 0, sm, status), f16_seen = w.bf16_tiles == 0;
+  bool ready = mbar_wait(&sm.q_ready[qt], 0, sm, status), f16_seen = bf16_tiles == 0;
   auto scores = [&](int t, int half) -> bool {
-    const bool bf16 = t < w.bf16_tiles;
+    const bool bf16 = t < bf16_tiles;
     if (half == 0) {
       bool ok = mbar_wait(&sm.k_full[t & 1], (t >> 1) & 1, sm, status);
       if (!bf16 && !f16_seen) {
@@ -395,19 +406,22 @@ __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Wor
     }
     const uint64_t k_desc = desc_k_major(smem_u32(sm.k[t & 1]) + half * (kHalfBytes / 2));
     const uint32_t id = idesc(bf16, false, 64);
+    if (leader) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint64_t at = ((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4;
-      mma_ss(col_s + half * 64, q_desc + at, k_desc + at, id, i > 0, leader);
+      for (int i = 0; i < 8; ++i) {
+        const uint64_t at = ((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4;
+        mma_ss(col_s + half * 64, q_desc + at, k_desc + at, id, i > 0);
+      }
+      mma_commit(&sm.s_full[s][half]);
+      if (half) mma_commit(&sm.k_empty[t & 1]);
     }
-    commit(&sm.s_full[s][half], leader);
-    if (half) commit(&sm.k_empty[t & 1], leader);
+    __syncwarp();
     return true;
   };
   ready = __all_sync(kAll, ready);
   bool ok = ready && first < tiles && scores(first, 0) && scores(first, 1);
   for (int t = first, u = 0; t < tiles && ok; t += stride, ++u) {
-    const bool bf16 = t < w.bf16_tiles;
+    const bool bf16 = t < bf16_tiles;
     ok = mbar_wait(&sm.v_full[t & 1], (t >> 1) & 1, sm, status);
     const uint32_t v = smem_u32(sm.v[t & 1]);
     const uint32_t id = idesc(bf16, bf16, 128);
@@ -417,15 +431,19 @@ __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Wor
       ok = ok && mbar_wait(&sm.p_ready[s][half], u & 1, sm, status);
       if (!__all_sync(kAll, ok)) { ok = false; break; }
       tc_fence_after();
+      if (leader) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mma_ts(col_o, col_s + half * 64 + i * 8, v_desc + half * step64 + i * step16, id, u > 0 || half > 0 || i > 0, leader);
-      commit(&sm.o_done[s], leader);
-      if (half) commit(&sm.v_empty[t & 1], leader);
+        for (int i = 0; i < 4; ++i)
+          mma_ts(col_o, col_s + half * 64 + i * 8, v_desc + half * step64 + i * step16, id, u > 0 || half > 0 || i > 0);
+        mma_commit(&sm.o_done[s]);
+        if (half) mma_commit(&sm.v_empty[t & 1]);
+      }
+      __syncwarp();
       if (t + stride < tiles && !scores(t + stride, half)) { ok = false; break; }
     }
   }
-  commit(&sm.all_done, leader);
+  if (leader) mma_commit(&sm.all_done);
+  __syncwarp();
 }
 
 // -- softmax -------------------------------------------------------------------------------------
@@ -549,14 +567,14 @@ __device__ __forceinline__ float max64(const uint32_t* raw) {
 
 // 64 scores -> probabilities, packed over the first half of `raw` and stored; their sums are added.
 template <bool BF16>
-__device__ __forceinline__ void exp64(uint32_t* raw, uint64_t scale, uint64_t minus_base, uint64_t (&sum)[2], uint32_t col_p) {
+__device__ __forceinline__ void exp64(uint32_t* raw, uint64_t scale, uint64_t minus_base, uint64_t (&sum)[4], uint32_t col_p) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     float x, y;
     unpair(fma2(pair(raw[2 * i], raw[2 * i + 1]), scale, minus_base), x, y);
     x = ex2(x);
     y = ex2(y);
-    sum[i & 1] = add2(sum[i & 1], pair(__float_as_uint(x), __float_as_uint(y)));
+    sum[i & 3] = add2(sum[i & 3], pair(__float_as_uint(x), __float_as_uint(y)));
     raw[i] = pack16(x, y, BF16);
   }
   tmem_st32(col_p, raw);
@@ -638,11 +656,11 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
           if (grows) m = now;
         }
         const uint64_t scale2 = pair(scale), minus_base = pair(-((m == -INFINITY ? 0.f : m) + offset));
-        uint64_t sum[2] = {0, 0};
+        uint64_t sum[4] = {0, 0, 0, 0};
         if (bf16) exp64<true>(raw, scale2, minus_base, sum, col_s + half * 64);
         else exp64<false>(raw, scale2, minus_base, sum, col_s + half * 64);
         float x, y;
-        unpair(add2(sum[0], sum[1]), x, y);
+        unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), x, y);
         l += x + y;
         tmem_st_wait();
       }
@@ -765,6 +783,7 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
     return;
   }
   if (threadIdx.x == 0) {
+    sm.work = w;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.k_full[i], 4);
       mbar_init(&sm.v_full[i], 4);
@@ -800,13 +819,16 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     RowState state{-INFINITY, 0.f};
     QueryRow q;
+    const Work w = sm.work;
     const bool ok = softmax(a, sm, w, tmem, stream, r, kvh, q, state);
     finish(a, sm, w, tmem, stream, r, q, state, split, ok);
   } else if (stream < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const Work w = sm.work;
     produce(a, sm, w, kvh, warp & 3, lane, stream == 3);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    const Work w = sm.work;
     if (warp < kIssueWarp + 2) {
       issue(a, sm, w, tmem, warp - kIssueWarp);
       // nothing of this CTA's is in flight when its tensor memory goes back, also after an expired wait

@@ -100,7 +100,7 @@ pool_fork_kernel(const PoolFork f, int pieces_per_run) {
     if (from < 0 || from >= f.slots || to < 0 || to >= f.slots || from == to) bad |= NVFP4_STATUS_BAD_TAIL_ID;
   }
   const int raw_fp4 = f.seqused_fp4[source];
-  const int pages = min(max(raw_fp4, 0) / kPage, f.columns);
+  const int pages = min(max(raw_fp4, 0) / kPage, min(max(f.pages_held[source], 0), f.columns));
   if (raw_fp4 != pages * kPage) bad |= NVFP4_STATUS_BAD_LENGTH;
   for (int c = threadIdx.x; c < pages; c += blockDim.x) {
     const int page = f.page_table[source * f.page_table_stride + c];

@@ -239,7 +239,8 @@ def fp4_chunk_attention(
         out: optional BF16 ``[>= tokens, heads_q, 128]``, dense within a token.
         lse: optional contiguous FP32 ``[>= tokens, heads_q]``: natural-log sum of the exponentials of the scaled scores.
         num_splits: ranges that each row's keys are cut into (None: by the launch's shape);
-            ``workspace``: their scratch, UINT8, ``chunk_workspace_bytes`` long (None: allocated).
+            ``workspace``: their scratch, UINT8, ``chunk_workspace_bytes`` long (None: allocated).  Calls, or
+            captured graphs, that share one must not run at the same time.
         status: one 32-bit integer on the device, a sticky OR of the ``NVFP4_STATUS_*`` bits.
         trusted_metadata: skip every check that reads device values back.
 

@@ -242,6 +242,19 @@ class LayerRuntime:
                 dtype=torch.int64, device=self.tail_key.device)
         return self._bases
 
+    def page_pool(self, kv_caches, *, refs: torch.Tensor | None = None, reserved_pages: int = 1):
+        """A :class:`pages.PagePool` over every layer's block array (``[blocks, bytes]``, layer order) and this model's
+        tails: forks, releases and compaction of what the layers hold.  Block 0 is vLLM's null block."""
+        from .pages import PagePool
+
+        kv_caches = [cache.view(torch.uint8) for cache in kv_caches]
+        if len(kv_caches) != self.num_layers:
+            raise ValueError(f"this model has {self.num_layers} layers, got {len(kv_caches)} block arrays")
+        for cache in kv_caches:
+            layout.carve(cache, self.num_kv_heads, self.head_dim)     # the shape the layers will read
+        return PagePool(kv_caches, refs=refs, tail_key=self.tail_key, tail_value=self.tail_value,
+                        reserved_pages=reserved_pages)
+
     def layer_regions(self, layer_index: int) -> tuple[torch.Tensor, ...]:
         return self._by_layer[layer_index]
 

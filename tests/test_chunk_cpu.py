@@ -59,6 +59,7 @@ def arguments(**changes):
 @pytest.mark.parametrize("entry", ["nvfp4_chunk_attention", "nvfp4_append_chunk"])
 @pytest.mark.parametrize("changes,words", [
     (dict(rows=-1), "negative"), (dict(tokens=-1), "negative"), (dict(rows=70000), "too many rows"),
+    (dict(max_chunk=5 << 20), "max_chunk"),
     (dict(heads_kv=0), "heads_kv"), (dict(seqused_fp4=None), "lengths"), (dict(chunk_start=None), "lengths"),
     (dict(key=None), "key and value"), (dict(key=SOME + 2), "16-byte"), (dict(key_token_stride=128), "dense within a token"),
     (dict(value_token_stride=260), "16-byte"), (dict(key_shift=SOME + 4), "16-byte"), (dict(k_sf=None), "non-null"),

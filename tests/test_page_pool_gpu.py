@@ -81,6 +81,12 @@ def test_fork_shares_pages_and_copies_tails(cuda_device, heads, seed):
     assert table.tolist() == t.tolist() and held.tolist() == h and pool.refs.tolist() == refs.tolist()
     assert full_d.tolist() == fp4 and used_d.tolist() == used
     assert torch.equal(pool.tail_key, tails[0]) and torch.equal(pool.tail_value, tails[1]) and int(pool.status) == 0
+    # a source whose sealed pages are more than it holds shares what it holds, and is flagged
+    pool.release(ints([5], cuda_device), table, held)
+    full_d[8] = (h[8] + 2) * 128
+    pool.fork(ints([8], cuda_device), ints([5], cuda_device), table, held, full_d, used_d, ints(slots, cuda_device))
+    assert int(pool.status) == L.STATUS_BAD_LENGTH and int(held[5]) == h[8] and int(full_d[5]) == h[8] * 128
+    pool.status.zero_()
     # pairs that would depend on an order are skipped and flagged: a target twice, a target that is a source
     before = (table.clone(), pool.refs.clone(), pool.tail_key.clone())
     pool.fork(ints([0, 5, 99], cuda_device), ints([5, 5, 1], cuda_device), table, held, full_d, used_d, ints(slots, cuda_device))
