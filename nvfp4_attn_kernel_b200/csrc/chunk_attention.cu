@@ -29,6 +29,8 @@
 // 128-row products and the operands' making: 32 rows x 4 tokens over 4096 tokens: 103 us for 160 MB.
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "chunk_common.cuh"
 #include "sm100_device.cuh"
 
@@ -881,8 +883,17 @@ template <int QTILES, int RAW>
 cudaError_t launch(const ChunkAttention& a, cudaStream_t stream) {
   const int bytes = (int)sizeof(ChunkSmem<QTILES, RAW>) + 1024;
   static_assert(sizeof(ChunkSmem<QTILES, RAW>) + 1024 <= 232448, "shared memory of one CTA");
-  cudaError_t e = cudaFuncSetAttribute(chunk_attention_kernel<QTILES, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  // once per device (the attribute belongs to the function on it)
+  static std::atomic<uint64_t> prepared{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device > 63 || !(prepared.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(chunk_attention_kernel<QTILES, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    prepared.fetch_or(bit, std::memory_order_release);
+  }
   ChunkMaps maps{};
   if (a.c.max_pages > 0 && a.c.num_pages > 0) {
     e = encode_map(0, a.c.k_packed, a.c.k_pitch, a.c.num_pages, a.c.heads_kv, &maps.k);

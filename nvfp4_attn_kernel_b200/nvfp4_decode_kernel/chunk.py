@@ -12,6 +12,7 @@ A step that continues sequences is :func:`fp4_chunk_attention` in every layer, t
 
 from __future__ import annotations
 
+import functools
 import math
 import struct
 
@@ -69,13 +70,14 @@ def _page_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, inde
     if key_scales.shape != want or value_scales.shape != want:
         raise ValueError(f"key_scales and value_scales must have shape {want}")
     k, ks, v, vs = key_pages_fp4.stride(), key_scales.stride(), value_pages_fp4.stride(), value_scales.stride()
-    if k[1:] != (heads * 64, 64, 1) or v[1:] != (HEAD_DIM * 64, 64, 1):
+    if k != (k[0], heads * 64, 64, 1) or v != (v[0], HEAD_DIM * 64, 64, 1):
         raise ValueError("key_pages_fp4 and value_pages_fp4 must be dense within a page")
-    if ks[1:] != (16, 4, 1024, 1, 512, 1024) or vs[1:] != (16, 4, 1024, 1, 512, 1024):
+    if ks != (ks[0], 16, 4, 1024, 1, 512, 1024) or vs != (vs[0], 16, 4, 1024, 1, 512, 1024):
         raise ValueError("key_scales and value_scales must use the quantisers' layout")
-    for tensor in (key_pages_fp4, key_scales, value_pages_fp4, value_scales):
-        if tensor.get_device() != index or tensor.element_size() != 1:
-            raise ValueError(f"the page regions must hold bytes on device {index}")
+    if not (key_pages_fp4.get_device() == key_scales.get_device() == value_pages_fp4.get_device()
+            == value_scales.get_device() == index and key_pages_fp4.itemsize == key_scales.itemsize
+            == value_pages_fp4.itemsize == value_scales.itemsize == 1):
+        raise ValueError(f"the page regions must hold bytes on device {index}")
     return (key_pages_fp4.data_ptr(), k[0], key_scales.data_ptr(), ks[0], value_pages_fp4.data_ptr(), v[0],
             value_scales.data_ptr(), vs[0]), pages, heads
 
@@ -169,6 +171,7 @@ def _check_metadata(table, seqused_fp4, starts, max_chunk_len, tokens, residual,
         raise ValueError("two chunks must not be appended to one page")
 
 
+@functools.lru_cache(maxsize=4096)      # of sizes alone
 def chunk_split_heuristic(rows: int, tokens: int, max_chunk_len: int, heads_q: int, heads_kv: int, max_pages: int, *,
                           sms: int) -> int:
     """Ranges that each row's keys are cut into, by predicted makespan.
@@ -404,7 +407,7 @@ def _sm_count(index: int) -> int:
 
 def _launch(call, index: int, *arguments) -> None:
     """A call of the library on the current stream of device ``index``."""
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         code = call(*arguments, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):

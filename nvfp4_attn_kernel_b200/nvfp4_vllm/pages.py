@@ -92,7 +92,7 @@ class PagePool:
 
     def _call(self, call, *args) -> None:
         index = self._index
-        if torch.cuda.current_device() == index:
+        if torch._C._cuda_getDevice() == index:
             code = call(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
             with torch.cuda.device(index):
