@@ -567,19 +567,94 @@ __device__ __forceinline__ float max64(const uint32_t* raw) {
   return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
-// 64 scores -> probabilities, packed over the first half of `raw` and stored; their sums are added.
+// 64 scores -> probabilities, packed over the first half of `raw` and stored; their sum is added to l.
 template <bool BF16>
-__device__ __forceinline__ void exp64(uint32_t* raw, uint64_t scale, uint64_t minus_base, uint64_t (&sum)[4], uint32_t col_p) {
+__device__ __forceinline__ void exp64(uint32_t* raw, float scale, float base, float& l, uint32_t col_p) {
+  const uint64_t scale2 = pair(scale), minus_base = pair(-base);
+  uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     float x, y;
-    unpair(fma2(pair(raw[2 * i], raw[2 * i + 1]), scale, minus_base), x, y);
+    unpair(fma2(pair(raw[2 * i], raw[2 * i + 1]), scale2, minus_base), x, y);
     x = ex2(x);
     y = ex2(y);
     sum[i & 3] = add2(sum[i & 3], pair(__float_as_uint(x), __float_as_uint(y)));
     raw[i] = pack16(x, y, BF16);
   }
   tmem_st32(col_p, raw);
+  float x, y;
+  unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), x, y);
+  l += x + y;
+}
+
+// Steps [first, last) of a stream, all over BF16 tiles or all over pages.
+template <bool BF16, class SM>
+__device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, const Work& w, uint32_t col_s, uint32_t col_o, int stream,
+                                              const QueryRow& q, bool warp_live, float scale, int first, int last, float& m, float& l) {
+  uint32_t* status = a.c.status;
+  constexpr uint32_t kAll = 0xffffffffu;
+  for (int u = first; u < last; ++u) {
+    const int t = w.two ? u : 2 * u + stream, tile = w.begin + t;
+    const float offset = BF16 && tile < w.fresh ? q.shift * scale : 0.f;
+    int limit = 128;
+    if (BF16) limit = tile < w.fresh ? q.token - tile * 128 + 1 : w.r.tail;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream][half], u & 1, sm, status))) return false;
+      tc_fence_after();
+      if (!BF16 && half == 0) limit = sm.page_ok[t & 7] ? 128 : 0;
+      if (half) limit -= 64;
+      if (warp_live) {
+        const uint32_t col = col_s + half * 64;
+        bool formed = false;
+        if (!__any_sync(kAll, limit < 64)) {
+          // The common half-step, on a path of its own (with the masks and the rescaling in line the compiler spends a
+          // quarter more time on the rest): nothing masked, no maximum that has grown too far.
+          uint32_t raw[64];
+          tmem_ld32(col, raw);
+          tmem_ld32(col + 32, raw + 32);
+          tmem_ld_wait();
+          if (!__any_sync(kAll, max64(raw) * scale - offset > m + kRescaleLog2)) {
+            exp64<BF16>(raw, scale, m + offset, l, col);
+            formed = true;
+          }
+        }
+        if (!formed) {
+          uint32_t raw[64];
+          tmem_ld32(col, raw);
+          tmem_ld32(col + 32, raw + 32);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 64; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
+          const float best = max64(raw);
+          const float now = best == -INFINITY ? -INFINITY : best * scale - offset;
+          const bool grows = now > m + kRescaleLog2;
+          if (__any_sync(kAll, grows)) {
+            const float alpha = grows ? ex2(m - now) : 1.f;       // 0 from an empty row
+            if (u > 0 || half > 0) {      // every product so far has to be in O: the last one is half-step 2 u + half - 1
+              if (!__all_sync(kAll, mbar_wait(&sm.o_done[stream], (half + 1) & 1, sm, status))) return false;
+              tc_fence_after();
+#pragma unroll 1
+              for (int i = 0; i < 8; ++i) {
+                uint32_t o[16];
+                tmem_ld16(col_o + i * 16, o);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                tmem_st16(col_o + i * 16, o);
+              }
+            }
+            l *= alpha;
+            if (grows) m = now;
+          }
+          exp64<BF16>(raw, scale, (m == -INFINITY ? 0.f : m) + offset, l, col);
+        }
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      mbar_arrive(&sm.p_ready[stream][half]);
+    }
+  }
+  return true;
 }
 
 template <class SM>
@@ -588,8 +663,9 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
   uint32_t* status = a.c.status;
   constexpr uint32_t kAll = 0xffffffffu;
   const int qt = w.two ? stream : 0;
+  uint8_t* query = sm.q[SM::kQTiles > 1 ? qt : 0];
   q = query_row(w, kvh, qt, r);
-  load_query(a, w, kvh, r, q, sm.q[SM::kQTiles > 1 ? qt : 0], w.two || stream == 0);
+  load_query(a, w, kvh, r, q, query, w.two || stream == 0);
   if (w.two || stream == 0) {
     fence_proxy_async();
     mbar_arrive(&sm.q_ready[qt]);
@@ -597,79 +673,25 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
   const uint32_t lanes = (uint32_t)(r & ~31) << 16;
   const uint32_t col_s = tmem + lanes + kColS + stream * 128, col_o = tmem + lanes + kColO + stream * 128;
   const bool warp_live = __any_sync(kAll, q.live);
-  // a score in log2 units: against the BF16 query, and against the row's FP16 form (never zero, so that a masked
-  // -inf stays -inf)
-  const float scale_bf16 = a.scale_log2;
-  const float scale_f16 = fmaxf(a.scale_log2 * exponent_value(q.exponent), 1.2e-38f);
   float m = -INFINITY, l = 0.f;
+  // this stream's steps over BF16 tiles, then those over pages; a score in log2 units is the product with the BF16
+  // query, or with the row's FP16 form, times a scale (never zero, so that a masked -inf stays -inf)
   const int steps = stream_steps(w, stream);
-  for (int u = 0; u < steps; ++u) {
-    const int t = w.two ? u : 2 * u + stream, tile = w.begin + t;
-    const bool bf16 = t < w.bf16_tiles;
-    const float scale = bf16 ? scale_bf16 : scale_f16;
-    const float offset = tile < w.fresh ? q.shift * scale : 0.f;
-    int limit = 128;
-#pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-      if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream][half], u & 1, sm, status))) return false;
-      tc_fence_after();
-      if (half == 0) {
-        limit = tile < w.fresh ? q.token - tile * 128 + 1 : bf16 ? w.r.tail : sm.page_ok[t & 7] ? 128 : 0;
-      } else {
-        limit -= 64;
-        if (t == w.bf16_tiles - 1 && w.bf16_tiles < w.end - w.begin) {
-          // the last product with the BF16 query: once the other stream's is done too where they share it (its next
-          // one waits for what follows), the rows become FP16
-          if (!w.two && t > 0 &&
-              !__all_sync(kAll, mbar_wait(&sm.s_full[stream ^ 1][1], ((t - 1) >> 1) & 1, sm, status)))
-            return false;
-          query_to_f16(sm.q[SM::kQTiles > 1 ? qt : 0], r, q.exponent);
-          fence_proxy_async();
-          mbar_arrive(&sm.q_f16[qt]);
-        }
-      }
-      if (warp_live) {
-        uint32_t raw[64];
-        tmem_ld32(col_s + half * 64, raw);
-        tmem_ld32(col_s + half * 64 + 32, raw + 32);
-        tmem_ld_wait();
-        if (__any_sync(kAll, limit < 64)) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
-        }
-        const float best = max64(raw);
-        const float now = best == -INFINITY ? -INFINITY : best * scale - offset;
-        const bool grows = now > m + kRescaleLog2;
-        if (__any_sync(kAll, grows)) {
-          const float alpha = grows ? ex2(m - now) : 1.f;       // 0 from an empty row
-          if (u > 0 || half > 0) {      // every product so far has to be in O: the last one is half-step 2 u + half - 1
-            if (!__all_sync(kAll, mbar_wait(&sm.o_done[stream], (half + 1) & 1, sm, status))) return false;
-            tc_fence_after();
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-              uint32_t o[16];
-              tmem_ld16(col_o + i * 16, o);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-              tmem_st16(col_o + i * 16, o);
-            }
-          }
-          l *= alpha;
-          if (grows) m = now;
-        }
-        const uint64_t scale2 = pair(scale), minus_base = pair(-((m == -INFINITY ? 0.f : m) + offset));
-        uint64_t sum[4] = {0, 0, 0, 0};
-        if (bf16) exp64<true>(raw, scale2, minus_base, sum, col_s + half * 64);
-        else exp64<false>(raw, scale2, minus_base, sum, col_s + half * 64);
-        float x, y;
-        unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), x, y);
-        l += x + y;
-        tmem_st_wait();
-      }
-      tc_fence_before();
-      mbar_arrive(&sm.p_ready[stream][half]);
-    }
+  const int bf16_steps = w.two ? w.bf16_tiles : (w.bf16_tiles + 1 - stream) >> 1;
+  if (!softmax_steps<true>(a, sm, w, col_s, col_o, stream, q, warp_live, a.scale_log2, 0, bf16_steps, m, l)) return false;
+  if (w.bf16_tiles > 0 && w.bf16_tiles < w.end - w.begin && (w.two || stream == ((w.bf16_tiles - 1) & 1))) {
+    // The last BF16 tile was this stream's: with its products - and, where the streams share the query, the other's
+    // last one, whose next waits for what follows - the rows become FP16.
+    if (!w.two && w.bf16_tiles > 1 &&
+        !__all_sync(kAll, mbar_wait(&sm.s_full[stream ^ 1][1], ((w.bf16_tiles - 2) >> 1) & 1, sm, status)))
+      return false;
+    query_to_f16(query, r, q.exponent);
+    fence_proxy_async();
+    mbar_arrive(&sm.q_f16[qt]);
   }
+  if (!softmax_steps<false>(a, sm, w, col_s, col_o, stream, q, warp_live,
+                            fmaxf(a.scale_log2 * exponent_value(q.exponent), 1.2e-38f), bf16_steps, steps, m, l))
+    return false;
   state.m = m;
   state.l = l;
   return true;
