@@ -598,7 +598,7 @@ __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, c
     const float offset = BF16 && tile < w.fresh ? q.shift * scale : 0.f;
     int limit = 128;
     if (BF16) limit = tile < w.fresh ? q.token - tile * 128 + 1 : w.r.tail;
-#pragma unroll 1
+#pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream][half], u & 1, sm, status))) return false;
       tc_fence_after();
