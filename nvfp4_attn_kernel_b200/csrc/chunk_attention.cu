@@ -74,7 +74,7 @@ struct ChunkSmem {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t q_ready[2], q_f16[2], s_full[2][2], p_ready[2][2], o_done[2], all_done;
   uint64_t raw_full[RAW], raw_empty[RAW];
-  float join[2][128];        // stream 1's maximum and sum, when the streams share a tile
+  float join[2][2][128];     // [stream] maximum and sum, when the streams share a tile; first the row's exponent and shift
   int page_ok[8];            // whether page tile t was fetched (0: a refused id), at t % 8: the fetch is at most six
                              // tiles ahead of the softmax
   uint32_t tmem_base;
@@ -454,8 +454,6 @@ __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Wor
 struct QueryRow {
   int token, head;       // of the chunk; query head
   bool live;
-  int exponent;          // see row_exponent
-  float shift;           // q . key_shift
 };
 
 __device__ __forceinline__ QueryRow query_row(const Work& w, int kvh, int tile, int r) {
@@ -464,61 +462,56 @@ __device__ __forceinline__ QueryRow query_row(const Work& w, int kvh, int tile, 
   q.token = w.token0 + tile * w.tile_tokens + in_tile;
   q.head = kvh * w.group + r - in_tile * w.group;
   q.live = in_tile < w.tile_tokens && q.token < w.r.n;
-  q.exponent = 127;
-  q.shift = 0.f;
   return q;
 }
 
-// Reads the row, finds its exponent and its product with the key shift, and (store) lays it out as an operand:
-// BF16, or FP16 at once when no K/V tile of the split is BF16.
-__device__ __forceinline__ void load_query(const ChunkAttention& a, const Work& w, int kvh, int r, QueryRow& q, uint8_t* dst,
-                                           bool store) {
+// The row becomes FP16 in place, scaled so that its largest magnitude is in [1, 2); returns the exponent.
+__device__ __forceinline__ int query_to_f16(uint8_t* tile, int r) {
   uint4 x[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = make_uint4(0, 0, 0, 0);
-  if (q.live) {
-    const uint16_t* src = a.query + (int64_t)(w.r.first + q.token) * a.q_token_stride + (int64_t)q.head * a.q_head_stride;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * 8);
-  }
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
+    x[i] = *reinterpret_cast<const uint4*>(tile + swizzled(r, i));
     top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu),
                                  __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
   }
-  q.exponent = row_exponent(max(top & 0xFFFFu, top >> 16));
-  if (a.c.key_shift && w.fresh > w.begin) {
-    const uint16_t* mu = a.c.key_shift + kvh * kHeadDim;
-    float even = 0.f, odd = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint4 y = *reinterpret_cast<const uint4*>(mu + i * 8);
-      float u[8], v[8];
-      unpack_bf16x8(x[i], u);
-      unpack_bf16x8(y, v);
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        even += u[j] * v[j];
-        odd += u[j + 1] * v[j + 1];
-      }
-    }
-    q.shift = even + odd;
-  }
-  if (!store) return;
-  const float f = exponent_value(254 - q.exponent);
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    *reinterpret_cast<uint4*>(dst + swizzled(r, i)) = w.bf16_tiles ? x[i] : bf16x8_to_f16x8(x[i], f);
-}
-
-__device__ __forceinline__ void query_to_f16(uint8_t* tile, int r, int exponent) {
+  const int exponent = row_exponent(max(top & 0xFFFFu, top >> 16));
   const float f = exponent_value(254 - exponent);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    uint4* at = reinterpret_cast<uint4*>(tile + swizzled(r, i));
-    *at = bf16x8_to_f16x8(*at, f);
+  for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(tile + swizzled(r, i)) = bf16x8_to_f16x8(x[i], f);
+  return exponent;
+}
+
+// Lays the warp's 32 rows out as an operand, in BF16, two whole rows of 256 bytes at a time.
+__device__ __forceinline__ void load_query(const ChunkAttention& a, const Work& w, int r, const QueryRow& q, uint8_t* tile) {
+  const int lane = r & 31;
+  const uint16_t* src = a.query + (int64_t)(w.r.first + q.token) * a.q_token_stride + (int64_t)q.head * a.q_head_stride;
+  const unsigned long long mine = q.live ? reinterpret_cast<unsigned long long>(src) : 0;
+  const uint32_t dst = smem_u32(tile) + swizzled((r & ~31) + (lane >> 4), lane & 15);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {      // row 2 i + (lane >> 4), and its place in the swizzle
+    const unsigned long long from = __shfl_sync(0xffffffffu, mine, i * 2 + (lane >> 4));
+    cp_async16((dst ^ ((2 * i & 7) << 4)) + i * 256, from ? reinterpret_cast<const uint16_t*>(from) + (lane & 15) * 8 : a.query,
+               from != 0);
   }
+  cp_async_commit();
+  cp_async_wait<0>();
+}
+
+__device__ __forceinline__ float dot_row(const uint8_t* tile, int r, const uint16_t* y) {
+  float even = 0.f, odd = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    float u[8], v[8];
+    unpack_bf16x8(*reinterpret_cast<const uint4*>(tile + swizzled(r, i)), u);
+    unpack_bf16x8(*reinterpret_cast<const uint4*>(y + i * 8), v);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      even += u[j] * v[j];
+      odd += u[j + 1] * v[j + 1];
+    }
+  }
+  return even + odd;
 }
 
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
@@ -590,15 +583,16 @@ __device__ __forceinline__ void exp64(uint32_t* raw, float scale, float base, fl
 // Steps [first, last) of a stream, all over BF16 tiles or all over pages.
 template <bool BF16, class SM>
 __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, const Work& w, uint32_t col_s, uint32_t col_o, int stream,
-                                              const QueryRow& q, bool warp_live, float scale, int first, int last, float& m, float& l) {
+                                              const QueryRow& q, float shift, bool warp_live, float scale, int first, int last, float& m, float& l) {
   uint32_t* status = a.c.status;
   constexpr uint32_t kAll = 0xffffffffu;
+  const bool two = SM::kQTiles > 1 && w.two;
   for (int u = first; u < last; ++u) {
-    const int t = w.two ? u : 2 * u + stream, tile = w.begin + t;
-    const float offset = BF16 && tile < w.fresh ? q.shift * scale : 0.f;
+    const int t = two ? u : 2 * u + stream, tile = w.begin + t;
+    const float offset = BF16 && tile < w.fresh ? shift * scale : 0.f;
     int limit = 128;
     if (BF16) limit = tile < w.fresh ? q.token - tile * 128 + 1 : w.r.tail;
-#pragma unroll
+#pragma unroll SM::kQTiles
     for (int half = 0; half < 2; ++half) {
       if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream][half], u & 1, sm, status))) return false;
       tc_fence_after();
@@ -659,80 +653,110 @@ __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, c
 
 template <class SM>
 __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int stream, int r,
-                                        int kvh, QueryRow& q, RowState& state) {
+                                        int kvh, RowState& state) {
   uint32_t* status = a.c.status;
   constexpr uint32_t kAll = 0xffffffffu;
-  const int qt = w.two ? stream : 0;
+  const bool two = SM::kQTiles > 1 && w.two;
+  const int qt = two ? stream : 0;
   uint8_t* query = sm.q[SM::kQTiles > 1 ? qt : 0];
-  q = query_row(w, kvh, qt, r);
-  load_query(a, w, kvh, r, q, query, w.two || stream == 0);
-  if (w.two || stream == 0) {
-    fence_proxy_async();
-    mbar_arrive(&sm.q_ready[qt]);
+  const QueryRow q = query_row(w, kvh, qt, r);
+  const bool warp_live = __any_sync(kAll, q.live);      // else the warp's rows are left as they are: nobody reads what comes of them
+  const bool loads = two || stream == 0, shifted = a.c.key_shift && w.fresh > w.begin;
+  int exponent = 127;
+  float shift = 0.f;
+  if (loads) {
+    if (warp_live) load_query(a, w, r, q, query);
+    if (w.bf16_tiles) {
+      fence_proxy_async();
+      mbar_arrive(&sm.q_ready[qt]);
+    }
+    __syncwarp();
+    if (warp_live && shifted) shift = dot_row(query, r, a.c.key_shift + kvh * kHeadDim);
+    if (w.bf16_tiles == 0) {
+      if (warp_live) exponent = query_to_f16(query, r);
+      if (!two) sm.join[0][0][r] = __int_as_float(exponent);
+      fence_proxy_async();
+      mbar_arrive(&sm.q_ready[qt]);
+      mbar_arrive(&sm.q_f16[qt]);
+    }
+  }
+  if (!two && shifted) {
+    if (stream == 0) sm.join[0][1][r] = shift;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    shift = sm.join[0][1][r];
   }
   const uint32_t lanes = (uint32_t)(r & ~31) << 16;
   const uint32_t col_s = tmem + lanes + kColS + stream * 128, col_o = tmem + lanes + kColO + stream * 128;
-  const bool warp_live = __any_sync(kAll, q.live);
   float m = -INFINITY, l = 0.f;
   // this stream's steps over BF16 tiles, then those over pages; a score in log2 units is the product with the BF16
   // query, or with the row's FP16 form, times a scale (never zero, so that a masked -inf stays -inf)
   const int steps = stream_steps(w, stream);
-  const int bf16_steps = w.two ? w.bf16_tiles : (w.bf16_tiles + 1 - stream) >> 1;
-  if (!softmax_steps<true>(a, sm, w, col_s, col_o, stream, q, warp_live, a.scale_log2, 0, bf16_steps, m, l)) return false;
-  if (w.bf16_tiles > 0 && w.bf16_tiles < w.end - w.begin && (w.two || stream == ((w.bf16_tiles - 1) & 1))) {
+  const int bf16_steps = two ? w.bf16_tiles : (w.bf16_tiles + 1 - stream) >> 1;
+  if (!softmax_steps<true>(a, sm, w, col_s, col_o, stream, q, shift, warp_live, a.scale_log2, 0, bf16_steps, m, l)) return false;
+  if (w.bf16_tiles > 0 && w.bf16_tiles < w.end - w.begin && (two || stream == ((w.bf16_tiles - 1) & 1))) {
     // The last BF16 tile was this stream's: with its products - and, where the streams share the query, the other's
     // last one, whose next waits for what follows - the rows become FP16.
-    if (!w.two && w.bf16_tiles > 1 &&
+    if (!two && w.bf16_tiles > 1 &&
         !__all_sync(kAll, mbar_wait(&sm.s_full[stream ^ 1][1], ((w.bf16_tiles - 2) >> 1) & 1, sm, status)))
       return false;
-    query_to_f16(query, r, q.exponent);
+    if (warp_live) exponent = query_to_f16(query, r);
+    if (!two) sm.join[0][0][r] = __int_as_float(exponent);
     fence_proxy_async();
     mbar_arrive(&sm.q_f16[qt]);
   }
-  if (!softmax_steps<false>(a, sm, w, col_s, col_o, stream, q, warp_live,
-                            fmaxf(a.scale_log2 * exponent_value(q.exponent), 1.2e-38f), bf16_steps, steps, m, l))
+  if (!two && bf16_steps < steps) {      // by the other stream, perhaps
+    if (!__all_sync(kAll, mbar_wait(&sm.q_f16[0], 0, sm, status))) return false;
+    exponent = __float_as_int(sm.join[0][0][r]);
+  }
+  if (!softmax_steps<false>(a, sm, w, col_s, col_o, stream, q, shift, warp_live,
+                            fmaxf(a.scale_log2 * exponent_value(exponent), 1.2e-38f), bf16_steps, steps, m, l))
     return false;
   state.m = m;
   state.l = l;
   return true;
 }
 
-// Rows out: divided by the sum, as BF16, or as a normalised fp32 partial with its log2-sum.
+// Rows out: divided by the sum, as BF16, or as a normalised fp32 partial with its log2-sum.  Streams that share a tile
+// finish half of the channels each and store them directly (a tile has few live rows then); else rows go through
+// shared memory, where a warp turns them into whole lines.
 template <class SM>
 __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int stream, int r,
-                                       const QueryRow& q, const RowState& state, int split, bool ok) {
+                                       int kvh, const RowState& state, int split, bool ok) {
   constexpr uint32_t kAll = 0xffffffffu;
-  const bool join = !w.two && w.steps > 1;      // stream 1 has a part of the same rows
+  const int lane = r & 31;
+  const bool two = SM::kQTiles > 1 && w.two;
+  const QueryRow q = query_row(w, kvh, two ? stream : 0, r);
+  const bool join = !two && w.steps > 1;      // the other stream has a part of the same rows
   ok = __all_sync(kAll, ok && mbar_wait(&sm.all_done, 0, sm, a.c.status));
   tc_fence_after();
   const uint32_t lanes = (uint32_t)(r & ~31) << 16;
   const uint32_t col_o = tmem + lanes + kColO + stream * 128;
+  const bool warp_live = __any_sync(kAll, q.live);
   float* shared_o = reinterpret_cast<float*>(sm.k);     // [channel][row]: every product has been formed
   if (join) {
-    if (stream == 1) {
-      if (ok) {
+    const int give = (stream ^ 1) * 64;
+    if (ok && warp_live) {
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          uint32_t o[32];
-          tmem_ld32(col_o + i * 32, o);
-          tmem_ld_wait();
+      for (int i = give; i < give + 64; i += 32) {
+        uint32_t o[32];
+        tmem_ld32(col_o + i, o);
+        tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) shared_o[(i * 32 + j) * 128 + r] = __uint_as_float(o[j]);
-        }
+        for (int j = 0; j < 32; ++j) shared_o[(i + j) * 128 + r] = __uint_as_float(o[j]);
       }
-      sm.join[0][r] = state.m;
-      sm.join[1][r] = state.l;
     }
+    sm.join[stream][0][r] = state.m;
+    sm.join[stream][1][r] = state.l;
     asm volatile("bar.sync 1, 256;" ::: "memory");
   }
-  if (!ok || sm.abort_flag || (!w.two && stream == 1)) return;
+  if (!ok || sm.abort_flag || !warp_live || (!two && !join && stream == 1)) return;
   float w0 = 1.f, w1 = 0.f, m = state.m, l = state.l;
   if (join) {
-    const float m1 = sm.join[0][r];
+    const float m1 = sm.join[stream ^ 1][0][r];
     m = fmaxf(state.m, m1);
     w0 = state.m == -INFINITY ? 0.f : ex2(state.m - m);
     w1 = m1 == -INFINITY ? 0.f : ex2(m1 - m);
-    l = state.l * w0 + sm.join[1][r] * w1;
+    l = state.l * w0 + sm.join[stream ^ 1][1][r] * w1;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   w0 *= inv;
@@ -740,32 +764,52 @@ __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Wo
   const int64_t token = (int64_t)w.r.first + q.token;
   const bool partial = a.num_splits > 1;
   const int64_t part = ((int64_t)split * a.c.tokens + token) * a.heads_q + q.head;
+  uint8_t* mine = partial ? reinterpret_cast<uint8_t*>(a.o_partial + part * kHeadDim)
+                          : reinterpret_cast<uint8_t*>(a.out + token * a.out_token_stride + q.head * kHeadDim);
+  const int begin = join ? stream * 64 : 0, end = join ? begin + 64 : kHeadDim;
+  const int bytes = partial ? 4 : 2, pass = 256 / bytes;      // channels that are staged at a time, 256 bytes of a row
+  uint8_t* stage = sm.v[stream];
 #pragma unroll 1
-  for (int i = 0; i < 4; ++i) {
+  for (int c = begin; c < end; c += 32) {
     uint32_t o[32];
     __syncwarp();
-    tmem_ld32(col_o + i * 32, o);
+    tmem_ld32(col_o + c, o);
     tmem_ld_wait();
     float x[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(o[j]) * w0;
     if (join) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] += shared_o[(i * 32 + j) * 128 + r] * w1;
+      for (int j = 0; j < 32; ++j) x[j] += shared_o[(c + j) * 128 + r] * w1;
     }
-    if (q.live && partial) {
-      float4* dst = reinterpret_cast<float4*>(a.o_partial + part * kHeadDim + i * 32);
+    const int first = (c & (pass - 1)) * bytes >> 4;
+    const auto put = [&](int unit, uint4 y) {
+      if (!join) *reinterpret_cast<uint4*>(stage + swizzled(r, first + unit)) = y;
+      else if (q.live) *reinterpret_cast<uint4*>(mine + c * bytes + unit * 16) = y;
+    };
+    if (partial) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dst[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-    } else if (q.live) {
-      uint4* dst = reinterpret_cast<uint4*>(a.out + token * a.out_token_stride + q.head * kHeadDim + i * 32);
+      for (int j = 0; j < 8; ++j)
+        put(j, make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), __float_as_uint(x[4 * j + 2]),
+                          __float_as_uint(x[4 * j + 3])));
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        dst[j] = make_uint4(pack16(x[8 * j], x[8 * j + 1], true), pack16(x[8 * j + 2], x[8 * j + 3], true),
-                            pack16(x[8 * j + 4], x[8 * j + 5], true), pack16(x[8 * j + 6], x[8 * j + 7], true));
+        put(j, make_uint4(pack16(x[8 * j], x[8 * j + 1], true), pack16(x[8 * j + 2], x[8 * j + 3], true),
+                          pack16(x[8 * j + 4], x[8 * j + 5], true), pack16(x[8 * j + 6], x[8 * j + 7], true)));
+    }
+    if (join || (c + 32 & (pass - 1))) continue;
+    __syncwarp();
+    const unsigned long long to = q.live ? reinterpret_cast<unsigned long long>(mine + (c + 32 - pass) * bytes) : 0;
+    const int unit = lane & 15, ahead = lane >> 4;
+    const uint32_t at = swizzled((r & ~31) + ahead, unit);
+#pragma unroll 8
+    for (int i = 0; i < 16; ++i) {            // row 2 i + ahead, and its place in the swizzle
+      uint4* dst = reinterpret_cast<uint4*>(__shfl_sync(kAll, to, 2 * i + ahead));
+      if (dst) dst[unit] = *reinterpret_cast<const uint4*>(stage + ((at ^ (2 * i & 7) << 4) + i * 256));
     }
   }
-  if (q.live) {
+  if (q.live && begin == 0) {
     const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
     if (partial) a.lse_partial[part] = lse2;
     else if (a.lse) a.lse[token * a.heads_q + q.head] = lse2 * kLn2;
@@ -775,44 +819,17 @@ __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Wo
 // grid (query blocks * splits, heads_kv, rows)
 template <int QTILES, int RAW>
 __global__ void __launch_bounds__(kThreads, 1)
-chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps maps, int query_blocks) {
+chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps maps, int query_blocks,
+                       int group, int tile_tokens) {
   using SM = ChunkSmem<QTILES, RAW>;
   extern __shared__ uint8_t smem_raw[];
   SM& sm = *reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int row = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the blocks with the longest causal reach first
-  const int split = blockIdx.x / query_blocks, block = query_blocks - 1 - (blockIdx.x - split * query_blocks);
-  Work w;
-  w.r = resolve_chunk_row(a.c, row, blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0);
-  w.group = a.heads_q / a.c.heads_kv;
-  w.tile_tokens = 128 / w.group;
-  w.token0 = block * QTILES * w.tile_tokens;
-  if (w.token0 >= w.r.n) return;
-  w.two = QTILES > 1 && w.token0 + w.tile_tokens < w.r.n;
-  const int last_token = min(w.r.n, w.token0 + (w.two ? 2 : 1) * w.tile_tokens);
-  w.fresh = (last_token + 127) >> 7;
-  w.tail_tiles = w.r.tail > 0;
-  const int tiles = w.fresh + w.tail_tiles + w.r.pages;
-  const int per = (tiles + a.num_splits - 1) / a.num_splits;
-  w.begin = min(split * per, tiles);
-  w.end = min(w.begin + per, tiles);
-  w.bf16_tiles = max(0, min(w.end, w.fresh + w.tail_tiles) - w.begin);
-  w.steps = (w.two ? 2 : 1) * (w.end - w.begin);
-  const int stream = warp >> 2, r = threadIdx.x & 127;
-  if (w.begin == w.end) {      // nothing in this range of the keys
-    if (stream < (w.two ? 2 : 1)) {
-      const QueryRow q = query_row(w, kvh, stream, r);
-      if (q.live) a.lse_partial[((int64_t)split * a.c.tokens + w.r.first + q.token) * a.heads_q + q.head] = -INFINITY;
-    }
-    return;
-  }
-  if (threadIdx.x == 0) {
-    sm.work = w;
+  // the barriers whose counts are known, while the row's lengths are on their way
+  if (threadIdx.x == kFetchWarp * 32) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.k_full[i], 4);
       mbar_init(&sm.v_full[i], 4);
-      mbar_init(&sm.k_empty[i], w.two ? 2 : 1);      // a tile serves both streams, or one
-      mbar_init(&sm.v_empty[i], w.two ? 2 : 1);
       mbar_init(&sm.s_full[i][0], 1);
       mbar_init(&sm.s_full[i][1], 1);
       mbar_init(&sm.p_ready[i][0], 128);
@@ -829,6 +846,40 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // the blocks with the longest causal reach first
+  const int split = a.num_splits == 1 ? 0 : blockIdx.x / query_blocks, block = query_blocks - 1 - (blockIdx.x - split * query_blocks);
+  Work w;
+  w.r = resolve_chunk_row(a.c, row, blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0);
+  w.group = group;
+  w.tile_tokens = tile_tokens;
+  w.token0 = block * QTILES * w.tile_tokens;
+  if (w.token0 >= w.r.n) return;
+  w.two = QTILES > 1 && w.token0 + w.tile_tokens < w.r.n;
+  const int last_token = min(w.r.n, w.token0 + (w.two ? 2 : 1) * w.tile_tokens);
+  w.fresh = (last_token + 127) >> 7;
+  w.tail_tiles = w.r.tail > 0;
+  const int tiles = w.fresh + w.tail_tiles + w.r.pages;
+  const int per = a.num_splits == 1 ? tiles : (tiles + a.num_splits - 1) / a.num_splits;
+  w.begin = min(split * per, tiles);
+  w.end = min(w.begin + per, tiles);
+  w.bf16_tiles = max(0, min(w.end, w.fresh + w.tail_tiles) - w.begin);
+  w.steps = (w.two ? 2 : 1) * (w.end - w.begin);
+  const int stream = warp >> 2, r = threadIdx.x & 127;
+  if (w.begin == w.end) {      // nothing in this range of the keys
+    if (stream < (w.two ? 2 : 1)) {
+      const QueryRow q = query_row(w, kvh, stream, r);
+      if (q.live) a.lse_partial[((int64_t)split * a.c.tokens + w.r.first + q.token) * a.heads_q + q.head] = -INFINITY;
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    sm.work = w;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.k_empty[i], w.two ? 2 : 1);      // a tile serves both streams, or one
+      mbar_init(&sm.v_empty[i], w.two ? 2 : 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem_base))
                  : "memory");
@@ -842,10 +893,9 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
   if (stream < 2) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     RowState state{-INFINITY, 0.f};
-    QueryRow q;
     const Work w = sm.work;
-    const bool ok = softmax(a, sm, w, tmem, stream, r, kvh, q, state);
-    finish(a, sm, w, tmem, stream, r, q, state, split, ok);
+    const bool ok = softmax(a, sm, w, tmem, stream, r, kvh, state);
+    finish(a, sm, w, tmem, stream, r, kvh, state, split, ok);
   } else if (stream < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const Work w = sm.work;
@@ -922,9 +972,10 @@ cudaError_t launch(const ChunkAttention& a, cudaStream_t stream) {
     if (e == cudaSuccess) e = encode_map(1, a.c.v_packed, a.c.v_pitch, a.c.num_pages, a.c.heads_kv, &maps.v);
     if (e != cudaSuccess) return e;
   }
-  const int tokens = 128 / (a.heads_q / a.c.heads_kv) * QTILES;
+  const int group = a.heads_q / a.c.heads_kv, tile_tokens = 128 / group, tokens = tile_tokens * QTILES;
   const int blocks = (a.c.max_chunk + tokens - 1) / tokens;
-  chunk_attention_kernel<QTILES, RAW><<<dim3(blocks * a.num_splits, a.c.heads_kv, a.c.rows), kThreads, bytes, stream>>>(a, maps, blocks);
+  chunk_attention_kernel<QTILES, RAW><<<dim3(blocks * a.num_splits, a.c.heads_kv, a.c.rows), kThreads, bytes, stream>>>(
+      a, maps, blocks, group, tile_tokens);
   return cudaGetLastError();
 }
 
