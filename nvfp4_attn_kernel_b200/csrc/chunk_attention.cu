@@ -926,6 +926,7 @@ constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(32 * kMergeWarps)
 chunk_merge_kernel(const ChunkAttention a) {
   const int lane = threadIdx.x & 31;
+  cudaGridDependencySynchronize();      // launched while the attention still runs (0.6 us of 18.9 at 16 tokens after 2048)
   const ChunkRow r = resolve_chunk_row(a.c, blockIdx.y, false);
   const int64_t unit = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
   const int i = (int)(unit / a.heads_q), head = (int)(unit - (int64_t)i * a.heads_q);
@@ -988,8 +989,16 @@ cudaError_t launch_chunk_attention(const ChunkAttention& a, cudaStream_t stream)
   cudaError_t e = a.c.max_chunk > tile_tokens ? launch<2, 3>(a, stream) : launch<1, 7>(a, stream);
   if (e != cudaSuccess || a.num_splits == 1) return e;
   const int64_t units = (int64_t)a.c.max_chunk * a.heads_q;
-  chunk_merge_kernel<<<dim3((unsigned)((units + kMergeWarps - 1) / kMergeWarps), a.c.rows), 32 * kMergeWarps, 0, stream>>>(a);
-  return cudaGetLastError();
+  cudaLaunchAttribute serial{};
+  serial.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  serial.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)((units + kMergeWarps - 1) / kMergeWarps), a.c.rows);
+  config.blockDim = dim3(32 * kMergeWarps);
+  config.stream = stream;
+  config.attrs = &serial;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, chunk_merge_kernel, a);
 }
 
 }  // namespace nvfp4
