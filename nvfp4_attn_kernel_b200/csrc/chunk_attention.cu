@@ -8,7 +8,7 @@
 //   - two tiles of query rows over the same K/V tiles, when the chunk has more than one, or
 //   - one tile of query rows whose K/V tiles the streams take in turns, joined at the end.
 // While one stream computes its softmax the tensor cores work for the other.  Beside the two softmax warpgroups one
-// makes K operands and one V operands (dequantising pages that a warp of their own fetches with tensor copies, or
+// makes K operands and one V operands (dequantising pages that a warp for each fetches with tensor copies, or
 // copying BF16 rows), a warp per stream issues the products.  Waits are bounded; an expired one sets a status bit.
 //
 // Operands.  A page's e2m1 * e4m3 is exact in FP16 (six significant bits, 2^-10 to 2688), and FP16
@@ -42,7 +42,7 @@ using namespace sm100;
 
 constexpr int kThreads = 640;         // warpgroups: softmax of two streams, K operands, V operands, issuers and fetch
 constexpr int kIssueWarp = 16;        // and 17: one per stream
-constexpr int kFetchWarp = 18;        // page bytes
+constexpr int kFetchWarp = 18;        // page bytes of K; 19: of V
 constexpr int kOperandBytes = 128 * 256;       // 128 rows of 128 16-bit elements: two 128-byte swizzled halves
 constexpr int kHalfBytes = 128 * 128;
 constexpr int kRawBytes = 8192 + 1024;         // a page's nibbles and scales for one head
@@ -75,8 +75,8 @@ struct ChunkSmem {
   uint64_t q_ready[2], q_f16[2], s_full[2][2], p_ready[2][2], o_done[2], all_done;
   uint64_t raw_full[RAW], raw_empty[RAW];
   float join[2][2][128];     // [stream] maximum and sum, when the streams share a tile; first the row's exponent and shift
-  int page_ok[8];            // whether page tile t was fetched (0: a refused id), at t % 8: the fetch is at most six
-                             // tiles ahead of the softmax
+  int page_ok[2][8];         // whether K's, V's page of tile t was fetched (0: a refused id), at t % 8: K's fetch is at
+                             // most seven tiles ahead of the softmax, V's five ahead of its operand
   uint32_t tmem_base;
   Work work;
   volatile int abort_flag;
@@ -270,61 +270,49 @@ struct Producer {
   }
 };
 
-// Page bytes into the raw slots, in the order K0 K1 V0 K2 V1 ... V(pages - 1): K a tile ahead of V, because an issuer
-// forms the next scores of its stream between the two halves of a tile's P V.  One tensor copy of the head's 128 x 64
-// bytes and one bulk copy of its scales each; page ids are fetched 32 at a time.
-template <class SM>
+// Page bytes into the raw slots of K, or of V: a warp each.  One tensor copy of the head's 128 x 64 bytes and one bulk
+// copy of its scales a page; page ids are fetched 32 at a time.  (One warp for both took 1400 clocks a tile, in which
+// short chunks could have had their products: 32 rows x 4 tokens after 4096 tokens 97 us, with two FETCHNEW.)
+template <bool V, class SM>
 __device__ __forceinline__ void fetch(const ChunkAttention& a, const ChunkMaps& maps, SM& sm, const Work& w, int row, int kvh,
                                       int lane) {
   constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int ring = V ? SM::kRawV : SM::kRawK, base = V ? SM::kRawK : 0;
   const ChunkCache& c = a.c;
-  const int pages = w.end - w.begin - w.bf16_tiles, items = 2 * pages;
+  const int pages = w.end - w.begin - w.bf16_tiles;
   const int32_t* table = c.page_table + (int64_t)row * c.page_table_row_stride + w.begin + w.bf16_tiles - w.fresh - w.tail_tiles;
-  int held_k = -1, held_v = -1, ids_k = 0, ids_v = 0;       // K and V are a tile apart: 32 ids each
-  int j = 0;
-  for (; j < items; ++j) {
-    const bool is_v = j == items - 1 || (j > 0 && !(j & 1));
-    const int p = j == items - 1 ? pages - 1 : is_v ? (j >> 1) - 1 : (j + 1) >> 1;
-    const int ring = is_v ? SM::kRawV : SM::kRawK, turn = p / ring, slot = p - turn * ring + (is_v ? SM::kRawK : 0);
-    if ((is_v ? held_v : held_k) != p >> 5) {
-      const int at = (p & ~31) + lane, id = at < pages ? table[at] : -1;
-      if (is_v) {
-        held_v = p >> 5;
-        ids_v = id;
-      } else {
-        held_k = p >> 5;
-        ids_k = id;
-      }
-    }
-    const int64_t page = __shfl_sync(kAll, is_v ? ids_v : ids_k, p & 31);
+  int ids = 0, slot = 0, p = 0;
+  uint32_t parity = 1;       // of the slot's last emptying
+  for (; p < pages; ++p) {
+    if (!(p & 31)) ids = p + lane < pages ? table[p + lane] : -1;
+    const int64_t page = __shfl_sync(kAll, ids, p & 31);
     const bool ok = page >= 0 && page < c.num_pages;
-    if (turn > 0 && !__all_sync(kAll, mbar_wait(&sm.raw_empty[slot], (turn - 1) & 1, sm, c.status))) break;
+    uint64_t* full = &sm.raw_full[base + slot];
+    if (p >= ring && !__all_sync(kAll, mbar_wait(&sm.raw_empty[base + slot], parity, sm, c.status))) break;
     if (lane == 0) {
-      if (!is_v) {
-        sm.page_ok[(w.bf16_tiles + p) & 7] = ok;
-        if (!ok) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
-      }
+      sm.page_ok[V][(w.bf16_tiles + p) & 7] = ok;
       if (ok) {
-        mbar_expect_tx(&sm.raw_full[slot], kRawBytes);
-        const uint32_t dst = smem_u32(sm.raw[slot]);
-        if (is_v) tma_load_4d(dst, &maps.v, &sm.raw_full[slot], 0, 0, kvh, (int)page);
-        else tma_load_4d(dst, &maps.k, &sm.raw_full[slot], 0, kvh, 0, (int)page);
-        bulk_load(dst + 8192, (is_v ? c.v_sf + page * c.v_sf_pitch : c.k_sf + page * c.k_sf_pitch) + kvh * kSfBlockBytes,
-                  kSfBlockBytes, &sm.raw_full[slot]);
+        mbar_expect_tx(full, kRawBytes);
+        const uint32_t dst = smem_u32(sm.raw[base + slot]);
+        if (V) tma_load_4d(dst, &maps.v, full, 0, 0, kvh, (int)page);
+        else tma_load_4d(dst, &maps.k, full, 0, kvh, 0, (int)page);
+        bulk_load(dst + 8192, (V ? c.v_sf + page * c.v_sf_pitch : c.k_sf + page * c.k_sf_pitch) + kvh * kSfBlockBytes,
+                  kSfBlockBytes, full);
       } else {
-        mbar_arrive(&sm.raw_full[slot]);
+        if (!V) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
+        mbar_arrive(full);
       }
     }
     __syncwarp();
+    if (++slot == ring) {
+      slot = 0;
+      parity ^= 1;
+    }
   }
   // nothing lands in shared memory after the CTA is gone, also after an expired wait: the last loads of each slot
   const unsigned long long t0 = global_ns();
-  const int fetched[2] = {j == 0 ? 0 : min((j >> 1) + 1, pages), j == items ? pages : j == 0 ? 0 : (j - 1) >> 1};
-  for (int v = 0; v < 2; ++v) {
-    const int ring = v ? SM::kRawV : SM::kRawK;
-    for (int p = max(0, fetched[v] - ring); p < fetched[v]; ++p)
-      while (!mbar_try(&sm.raw_full[p % ring + (v ? SM::kRawK : 0)], (p / ring) & 1) && global_ns() - t0 < 200000000ull) {}
-  }
+  for (int q = max(0, p - ring); q < p; ++q)
+    while (!mbar_try(&sm.raw_full[base + q % ring], (q / ring) & 1) && global_ns() - t0 < 200000000ull) {}
 }
 
 // One warpgroup makes the K operands, one the V operands.
@@ -359,7 +347,7 @@ __device__ __forceinline__ void produce(const ChunkAttention& a, SM& sm, const W
   }
   for (int t = w.bf16_tiles; t < tiles; ++t) {      // pages: through this operand's ring of raw slots
     if (!__all_sync(0xffffffffu, mbar_wait(&sm.raw_full[slot], parity, sm, a.c.status) && wait_empty(t))) goto out;
-    p.expand(sm.raw[slot], stage[t & 1], sm.page_ok[t & 7] != 0);
+    p.expand(sm.raw[slot], stage[t & 1], sm.page_ok[is_v][t & 7] != 0);
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.raw_empty[slot]);
     hand_over(t);
@@ -596,7 +584,7 @@ __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, c
     for (int half = 0; half < 2; ++half) {
       if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream][half], u & 1, sm, status))) return false;
       tc_fence_after();
-      if (!BF16 && half == 0) limit = sm.page_ok[t & 7] ? 128 : 0;
+      if (!BF16 && half == 0) limit = sm.page_ok[0][t & 7] ? 128 : 0;
       if (half) limit -= 64;
       if (warp_live) {
         const uint32_t col = col_s + half * 64;
@@ -910,7 +898,9 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
       while (!mbar_try(&sm.all_done, 0) && global_ns() - t0 < 200000000ull) {}
       __syncwarp();
     } else if (warp == kFetchWarp) {
-      fetch(a, maps, sm, w, row, kvh, lane);
+      fetch<false>(a, maps, sm, w, row, kvh, lane);
+    } else {
+      fetch<true>(a, maps, sm, w, row, kvh, lane);
     }
   }
   tc_fence_before();
