@@ -23,10 +23,12 @@
 // rescaled then; probabilities up to 2^8 fit both formats with the same relative precision).  A chunk token whose
 // value is not finite makes earlier tokens of its 128-token tile not finite too (0 * inf in the product).
 //
-// What bounds it: long chunks, the softmax warpgroups (exponentials: 2048 of about 4600 clocks per pair of tiles, which
-// the two streams spend side by side; with the softmax left out the same products run at 1430 TFLOP/s).  1152 tokens of
-// 32 / 8 heads over 16384 tokens: 335 us = 954 TFLOP/s, 0.58 of a large library product's burst rate.  Short chunks, the
-// 128-row products and the operands' making: 32 rows x 4 tokens over 4096 tokens: 103 us for 160 MB.
+// What bounds it: long chunks, the softmax warpgroups (exponentials: 2048 of about 3900 clocks per pair of tiles, in
+// which the products take 2048 too; with the softmax left out they run at 1430 TFLOP/s).  1152 tokens of 32 / 8 heads
+// over 16384 tokens: 282 us = 1135 TFLOP/s, 0.69 of a large library product's burst rate.  A CTA spends about 10 us before
+// and after its tiles (query rows in, the first products, rows out).  Short chunks: 128-row products for a few live rows
+// (1024 clocks a tile) and a tile's way through dequantisation, scores, softmax and P V, 1750 clocks a tile: 32 rows x 4
+// tokens over 4096 tokens 87 us for 160 MB.
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -56,6 +58,7 @@ struct Work {
   int group, tile_tokens;      // query heads per KV head; tokens in a tile of query rows
   int token0;                  // first chunk token of tile 0
   bool two;                    // two tiles of query rows; else one, the streams taking turns
+  bool apart;                  // one tile of at most 64 rows: rows 0..63 are stream 0's, their copies 64..127 stream 1's
   int fresh, tail_tiles;       // K/V tiles: the chunk's, then the tail's (0 or 1), then the pages
   int begin, end;              // this split's range of them
   int bf16_tiles;              // of these, how many are BF16
@@ -271,8 +274,8 @@ struct Producer {
 };
 
 // Page bytes into the raw slots of K, or of V: a warp each.  One tensor copy of the head's 128 x 64 bytes and one bulk
-// copy of its scales a page; page ids are fetched 32 at a time.  (One warp for both took 1400 clocks a tile, in which
-// short chunks could have had their products: 32 rows x 4 tokens after 4096 tokens 97 us, with two FETCHNEW.)
+// copy of its scales a page; page ids are fetched 32 at a time.  (One warp for both took 1400 clocks a tile,
+// longer than the tile's products: 18 rows x 30 tokens after 8192 tokens 94 us, with two 89 us.)
 template <bool V, class SM>
 __device__ __forceinline__ void fetch(const ChunkAttention& a, const ChunkMaps& maps, SM& sm, const Work& w, int row, int kvh,
                                       int lane) {
@@ -438,17 +441,17 @@ __device__ __forceinline__ void issue(const ChunkAttention& a, SM& sm, const Wor
 
 // -- softmax -------------------------------------------------------------------------------------
 
-// A thread's query row.
+// A thread's query row (tile row r).
 struct QueryRow {
   int token, head;       // of the chunk; query head
   bool live;
 };
 
-__device__ __forceinline__ QueryRow query_row(const Work& w, int kvh, int tile, int r) {
+__device__ __forceinline__ QueryRow query_row(const Work& w, int kvh, int tile, int r, bool apart = false) {
   QueryRow q;
-  const int in_tile = r / w.group;
+  const int index = apart ? r & 63 : r, in_tile = index / w.group;
   q.token = w.token0 + tile * w.tile_tokens + in_tile;
-  q.head = kvh * w.group + r - in_tile * w.group;
+  q.head = kvh * w.group + index - in_tile * w.group;
   q.live = in_tile < w.tile_tokens && q.token < w.r.n;
   return q;
 }
@@ -647,21 +650,23 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
   const bool two = SM::kQTiles > 1 && w.two;
   const int qt = two ? stream : 0;
   uint8_t* query = sm.q[SM::kQTiles > 1 ? qt : 0];
-  const QueryRow q = query_row(w, kvh, qt, r);
-  const bool warp_live = __any_sync(kAll, q.live);      // else the warp's rows are left as they are: nobody reads what comes of them
+  const bool apart = SM::kQTiles == 1 && w.apart;
+  const QueryRow q = query_row(w, kvh, qt, r, apart);
+  // rows that no query has are left as they are: nobody reads what comes of them
+  const bool warp_loads = __any_sync(kAll, q.live), warp_live = warp_loads && (!apart || r >> 6 == stream);
   const bool loads = two || stream == 0, shifted = a.c.key_shift && w.fresh > w.begin;
   int exponent = 127;
   float shift = 0.f;
   if (loads) {
-    if (warp_live) load_query(a, w, r, q, query);
+    if (warp_loads) load_query(a, w, r, q, query);
     if (w.bf16_tiles) {
       fence_proxy_async();
       mbar_arrive(&sm.q_ready[qt]);
     }
     __syncwarp();
-    if (warp_live && shifted) shift = dot_row(query, r, a.c.key_shift + kvh * kHeadDim);
+    if (warp_loads && shifted) shift = dot_row(query, r, a.c.key_shift + kvh * kHeadDim);
     if (w.bf16_tiles == 0) {
-      if (warp_live) exponent = query_to_f16(query, r);
+      if (warp_loads) exponent = query_to_f16(query, r);
       if (!two) sm.join[0][0][r] = __int_as_float(exponent);
       fence_proxy_async();
       mbar_arrive(&sm.q_ready[qt]);
@@ -687,7 +692,7 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
     if (!two && w.bf16_tiles > 1 &&
         !__all_sync(kAll, mbar_wait(&sm.s_full[stream ^ 1][1], ((w.bf16_tiles - 2) >> 1) & 1, sm, status)))
       return false;
-    if (warp_live) exponent = query_to_f16(query, r);
+    if (warp_loads) exponent = query_to_f16(query, r);
     if (!two) sm.join[0][0][r] = __int_as_float(exponent);
     fence_proxy_async();
     mbar_arrive(&sm.q_f16[qt]);
@@ -713,7 +718,10 @@ __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Wo
   constexpr uint32_t kAll = 0xffffffffu;
   const int lane = r & 31;
   const bool two = SM::kQTiles > 1 && w.two;
-  const QueryRow q = query_row(w, kvh, two ? stream : 0, r);
+  const bool apart = SM::kQTiles == 1 && w.apart;
+  QueryRow q = query_row(w, kvh, two ? stream : 0, r, apart);
+  if (apart && r >> 6 != stream) q.live = false;
+  const int other = apart ? r ^ 64 : r;       // the same query in the other stream
   const bool join = !two && w.steps > 1;      // the other stream has a part of the same rows
   ok = __all_sync(kAll, ok && mbar_wait(&sm.all_done, 0, sm, a.c.status));
   tc_fence_after();
@@ -740,11 +748,11 @@ __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Wo
   if (!ok || sm.abort_flag || !warp_live || (!two && !join && stream == 1)) return;
   float w0 = 1.f, w1 = 0.f, m = state.m, l = state.l;
   if (join) {
-    const float m1 = sm.join[stream ^ 1][0][r];
+    const float m1 = sm.join[stream ^ 1][0][other];
     m = fmaxf(state.m, m1);
     w0 = state.m == -INFINITY ? 0.f : ex2(state.m - m);
     w1 = m1 == -INFINITY ? 0.f : ex2(m1 - m);
-    l = state.l * w0 + sm.join[stream ^ 1][1][r] * w1;
+    l = state.l * w0 + sm.join[stream ^ 1][1][other] * w1;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   w0 *= inv;
@@ -768,7 +776,7 @@ __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Wo
     for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(o[j]) * w0;
     if (join) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] += shared_o[(c + j) * 128 + r] * w1;
+      for (int j = 0; j < 32; ++j) x[j] += shared_o[(c + j) * 128 + other] * w1;
     }
     const int first = (c & (pass - 1)) * bytes >> 4;
     const auto put = [&](int unit, uint4 y) {
@@ -852,6 +860,9 @@ chunk_attention_kernel(const ChunkAttention a, const __grid_constant__ ChunkMaps
   w.end = min(w.begin + per, tiles);
   w.bf16_tiles = max(0, min(w.end, w.fresh + w.tail_tiles) - w.begin);
   w.steps = (w.two ? 2 : 1) * (w.end - w.begin);
+  // (so that the streams' softmax warps are on different quarters of the SM: 32 rows x 4 tokens after 4096 tokens, 16
+  // query rows a tile, 97 us with both streams on the same warps' rows, 87 us apart)
+  w.apart = QTILES == 1 && w.steps > 1 && (w.r.n - w.token0) * group <= 64;
   const int stream = warp >> 2, r = threadIdx.x & 127;
   if (w.begin == w.end) {      // nothing in this range of the keys
     if (stream < (w.two ? 2 : 1)) {

@@ -177,8 +177,8 @@ def chunk_split_heuristic(rows: int, tokens: int, max_chunk_len: int, heads_q: i
     """Ranges that each row's keys are cut into, by predicted makespan.
 
     A CTA takes one KV head of one row and a block of query rows (one tile of 128 query rows, two where a chunk has
-    more), one CTA per SM.  It costs about 10 us before and after its K/V tiles and 1.05 us a tile with one query tile,
-    2.1 with two (measured: 32 rows x 4 tokens after 4096 tokens 96 us in two waves of 33 tiles, 512 tokens after 16384
+    more), one CTA per SM.  It costs about 10 us before and after its K/V tiles and 0.95 us a tile with one query tile,
+    2.1 with two (measured: 32 rows x 4 tokens after 4096 tokens 87 us in two waves of 33 tiles, 512 tokens after 16384
     270 us); a split adds a launch of 3 us and its partial results' way through memory.  The table's width stands for
     the lengths, which the host does not know.  Only counts that just fill a number of waves are tried; one that is
     not a twentieth faster than whole rows is not taken.  Over twelve shapes of 1 to 777 tokens after 0 to 32768 the
@@ -187,7 +187,7 @@ def chunk_split_heuristic(rows: int, tokens: int, max_chunk_len: int, heads_q: i
     if rows < 1 or tokens < 1 or max_chunk_len < 1 or sms < 1:
         return 1
     tile = 128 // (heads_q // heads_kv)
-    per, tile_us = (tile, 1.05) if max_chunk_len <= tile else (2 * tile, 2.1)
+    per, tile_us = (tile, 0.95) if max_chunk_len <= tile else (2 * tile, 2.1)
     ctas = min(rows * -(-max_chunk_len // per), tokens // per + rows) * heads_kv
     tiles = max_pages + -(-max_chunk_len // 128)
     best, best_us = 1, 0.95 * -(-ctas // sms) * (10.0 + tiles * tile_us)
