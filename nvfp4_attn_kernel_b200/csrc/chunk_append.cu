@@ -15,11 +15,12 @@ namespace nvfp4 {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kTileWords = 65;   // a token's 128 bf16 as 64 words, one word of padding
+// Word of channel pair `pair` of a token in the V tile: one word of padding a token, and four more per group of 16
+// tokens, so that a warp that reads four pairs of a token of each group has every lane in a bank of its own.
+__device__ __forceinline__ int tile_word(int tok, int pair) { return tok * 65 + (tok >> 4) * 4 + pair; }
 
 struct AppendSmem {
-  uint32_t tile[kPage * kTileWords];             // V: [token][channel pairs]
-  __align__(16) uint8_t packed[kHeadDim * 64];   // V: [channel][64 B]
+  uint32_t tile[kPage * 65 + 7 * 4];             // V: [token][channel pairs]
   __align__(16) uint8_t scales[kSfBlockBytes];
 };
 
@@ -102,38 +103,43 @@ __device__ __forceinline__ void seal_value(const ChunkCache& c, const ChunkRow& 
     }
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      uint32_t* dst = sm.tile + (tok0 + k * (kAppendThreads / 8)) * kTileWords + g * 8;
+      uint32_t* dst = sm.tile + tile_word(tok0 + k * (kAppendThreads / 8), g * 8);
       dst[0] = a[k].x; dst[1] = a[k].y; dst[2] = a[k].z; dst[3] = a[k].w;
       dst[4] = b[k].x; dst[5] = b[k].y; dst[6] = b[k].z; dst[7] = b[k].w;
     }
   }
   __syncthreads();
+  // a thread takes 16 tokens of two neighbouring channels; eight lanes store the 64 bytes of a channel
+  uint8_t* packed = c.v_packed + page * c.v_pitch + (int64_t)head * kHeadDim * 64;
+  const int g = threadIdx.x & 7;
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int it = threadIdx.x + k * kAppendThreads;
-    const int g = it >> 7, d = it & 127;
-    float x[16];
+  for (int k = 0; k < kItems / 2; ++k) {
+    const int pair = (threadIdx.x >> 3) + k * (kAppendThreads / 8);
+    float even[16], odd[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const uint32_t w = sm.tile[(g * 16 + i) * kTileWords + (d >> 1)];
-      x[i] = (d & 1) ? __uint_as_float(w & 0xFFFF0000u) : __uint_as_float(w << 16);
+      const uint32_t w = sm.tile[tile_word(g * 16 + i, pair)];
+      even[i] = __uint_as_float(w << 16);
+      odd[i] = __uint_as_float(w & 0xFFFF0000u);
     }
     uint32_t lo, hi;
     uint8_t s;
-    quantize_group16(x, lo, hi, s);
-    *reinterpret_cast<uint2*>(sm.packed + d * 64 + g * 8) = make_uint2(lo, hi);
-    sm.scales[sf_offset(d, g)] = s;
+    quantize_group16(even, lo, hi, s);
+    *reinterpret_cast<uint2*>(packed + 2 * pair * 64 + g * 8) = make_uint2(lo, hi);
+    sm.scales[sf_offset(2 * pair, g)] = s;
+    quantize_group16(odd, lo, hi, s);
+    *reinterpret_cast<uint2*>(packed + (2 * pair + 1) * 64 + g * 8) = make_uint2(lo, hi);
+    sm.scales[sf_offset(2 * pair + 1, g)] = s;
   }
   __syncthreads();
-  uint4* packed = reinterpret_cast<uint4*>(c.v_packed + page * c.v_pitch + (int64_t)head * kHeadDim * 64);
   uint4* scales = reinterpret_cast<uint4*>(c.v_sf + page * c.v_sf_pitch + head * kSfBlockBytes);
-  for (int i = threadIdx.x; i < kHeadDim * 64 / 16; i += kAppendThreads)
-    packed[i] = reinterpret_cast<const uint4*>(sm.packed)[i];
   if (threadIdx.x < kSfBlockBytes / 16) scales[threadIdx.x] = reinterpret_cast<const uint4*>(sm.scales)[threadIdx.x];
 }
 
-// grid (heads_kv * 2, columns, rows)
-__global__ void __launch_bounds__(kAppendThreads)
+// grid (heads_kv * 2, columns, rows).  512 bytes in and 144 out per token and head, bound by the loads in flight: 64
+// registers, so four CTAs an SM: 8 rows x 2048 tokens of 8 heads 19.2 us (61 MB, 3.2 TB/s); 80 registers and three CTAs
+// 20.3 us, 48 and five (with spills) 22.4 us.  4 rows x 5 tokens: 2.0 us, a launch and two loads that follow one another.
+__global__ void __launch_bounds__(kAppendThreads, 4)
 append_chunk_kernel(const ChunkCache c, int32_t* seqused_fp4_out, int32_t* seqused_tail_out) {
   __shared__ AppendSmem sm;
   const int row = blockIdx.z, column = blockIdx.y;
@@ -226,7 +232,8 @@ __device__ __forceinline__ int out_word(int tok, int pair) { return tok * kOutWo
 
 // grid (pages, heads_kv * 2).  K rows are rows of the result: four bytes in, sixteen out per thread.  V is packed along the
 // tokens: a thread takes 32 tokens of two neighbouring channels, and the page is turned in shared memory.  Bound by
-// memory: 144 bytes in and 512 out per token and head.
+// memory: 144 bytes in and 512 out per token and head; 256 pages of 8 heads 32 us (5.4 TB/s), 90
+// pages just written 9.7 us (6.3 TB/s).
 __global__ void __launch_bounds__(kAppendThreads)
 dequantize_pages_kernel(const ChunkCache c, const int32_t* __restrict__ page_ids, uint16_t* __restrict__ key_out,
                         uint16_t* __restrict__ value_out) {

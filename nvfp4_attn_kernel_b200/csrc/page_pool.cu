@@ -4,6 +4,10 @@
 // Compaction moves the live pages into the lowest ids: with L live pages, the k-th live page at or
 // above L goes to the k-th free id below L, so sources and destinations never meet, every page is
 // moved by whoever gets to it, and the result does not depend on any order.
+//
+// Bound by memory where pages or tails move (a thread has four 16-byte loads in flight, eight CTAs an SM): forks of 40
+// rows x 32 layers 105 us (6.9 TB/s read and written), a compaction of 1500 pages in 8 layers 140 us (5.4 TB/s).
+// Small calls are a launch or two: three forks of one KV head 4.7 us, a compaction of 300 pages in one layer 8 us.
 #include "chunk_common.cuh"
 
 namespace nvfp4 {
