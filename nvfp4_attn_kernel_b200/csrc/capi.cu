@@ -840,8 +840,16 @@ int nvfp4_append_chunk(const nvfp4_chunk_args* a, void* stream) {
   if (a->rows == 0) return NVFP4_OK;
   if (!a->seqused_fp4_out || !a->seqused_tail_out)
     return fail(NVFP4_ERR_INVALID, "append_chunk: the lengths afterwards need buffers");
-  if (a->seqused_fp4_out == a->seqused_fp4 || a->seqused_tail_out == a->seqused_tail ||
-      a->seqused_fp4_out == a->seqused_tail || a->seqused_tail_out == a->seqused_fp4)
+  // (the rows' CTAs read the lengths while one of them writes the new ones)
+  const auto apart = [&](const int32_t* x, const int32_t* y, int64_t count_y) {
+    const auto from_x = reinterpret_cast<uintptr_t>(x), from_y = reinterpret_cast<uintptr_t>(y);
+    return from_x + 4 * (uintptr_t)a->rows <= from_y || from_y + 4 * (uintptr_t)count_y <= from_x;
+  };
+  bool own = apart(a->seqused_fp4_out, a->seqused_tail_out, a->rows);
+  for (const int32_t* out : {a->seqused_fp4_out, a->seqused_tail_out})
+    own = own && apart(out, a->seqused_fp4, a->rows) && apart(out, a->seqused_tail, a->rows) &&
+          apart(out, a->tail_ids, a->rows) && apart(out, a->chunk_start, (int64_t)a->rows + 1);
+  if (!own)
     return fail(NVFP4_ERR_INVALID, "append_chunk: the lengths afterwards need buffers of their own");
   cudaError_t e = nvfp4::launch_append_chunk(c, a->seqused_fp4_out, a->seqused_tail_out,
                                              static_cast<cudaStream_t>(stream));

@@ -153,3 +153,14 @@ def test_operators_refuse_host_tensors():
         dequantize_pages(z, z, z, z, z)
     with pytest.raises(ValueError, match="UINT8 CUDA"):
         PagePool([torch.zeros(4, 32, dtype=torch.uint8)])
+
+
+@pytest.mark.parametrize("changes", [
+    dict(seqused_fp4_out=SOME + 16 + 4), dict(seqused_fp4_out=SOME + 16 - 4), dict(seqused_tail_out=SOME + 48),
+    dict(seqused_tail_out=SOME + 48 + 4), dict(seqused_tail_out=SOME + 32 + 4), dict(seqused_fp4_out=SOME + 8),
+    dict(seqused_tail_out=SOME - 4)])
+def test_append_refuses_overlapping_lengths(changes):
+    """Lengths that are written over ones that are read (shifted by one entry, the other output, the chunk's starts,
+    the residual ids), with two rows."""
+    assert L.load().nvfp4_append_chunk(ctypes.byref(arguments(**changes)), None) == L.ERR_INVALID
+    assert "of their own" in L.last_error()
