@@ -58,6 +58,37 @@ def test_attention_split_over_the_keys(cuda_device, splits):
     assert (out[-2:] == 3.0).all() and (lse[-2:] == 3.0).all()
 
 
+@pytest.mark.parametrize("splits", [1, 2, 5])
+@pytest.mark.parametrize("heads,lengths", [((8, 2), (15, 16, 17)), ((6, 2), (20, 21, 22)), ((8, 1), (7, 8, 9)),
+                                           ((32, 1), (1, 2, 3)), ((4, 4), (63, 64, 65, 128))],
+                         ids=["4to1", "3to1", "8to1", "32to1", "1to1"])
+def test_attention_around_half_a_tile(cuda_device, heads, lengths, splits):
+    """Just below, at and above 64 query rows of a KV head (up to there a tile holds each twice), over the chunk alone, a
+    tail, pages, and both; split, the ranges are of one tile and less."""
+    rows = [(f, t, n) for n in lengths for f, t in ((0, 0), (0, 5), (1, 0), (2, 128), (5, 9))]
+    batch = ChunkBatch(rows, *heads, cuda_device, seed=31, shift=heads[1] == 2)
+    lse = torch.empty(batch.tokens, heads[0], device=cuda_device)
+    check(batch, batch.attend(num_splits=splits, lse=lse), lse)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("chunk", [3, 70])
+def test_attention_leaves_refused_pages_out(cuda_device, chunk, splits):
+    """Ids outside the cache among 75 pages (the first, the last of 32, the first of the next 32, neighbours, the last):
+    what a table without them gives, and a status bit."""
+    batch = ChunkBatch([(75, 20, chunk), (40, 0, 1)], 8, 2, cuda_device, seed=32, shift=True)
+    refused = [0, 31, 32, 40, 41, 42, 74]
+    batch.table[0, refused] = torch.tensor([-1, 1 << 30, -5, 1 << 28, -1, batch.cache.shape[0], -1], dtype=torch.int32,
+                                           device=cuda_device)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    out = batch.attend(num_splits=splits, status=status, trusted_metadata=True)
+    assert int(status) == L.STATUS_BAD_PAGE_ID
+    kept = [c for c in range(75) if c not in refused]
+    batch.table_host[0, :len(kept)] = batch.table_host[0, kept].clone()
+    batch.rows[0] = (len(kept), 20, chunk)
+    check(batch, out)
+
+
 def test_attention_of_strided_projections(cuda_device):
     batch = ChunkBatch(EDGES, 8, 2, cuda_device, seed=5, spread=True)
     wide = torch.zeros(batch.tokens, 8 * 128 + 256, dtype=torch.bfloat16, device=cuda_device)
