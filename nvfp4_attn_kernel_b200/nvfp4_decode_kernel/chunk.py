@@ -250,6 +250,8 @@ def fp4_chunk_attention(
 
     The chunk is read from ``key`` / ``value`` in BF16 whether or not it has been appended already; ``seqused_*``
     are the lengths before it.  Unlike ``fp4_decode`` the query and the probabilities are not quantised.
+    A key that a token does not see does not reach it, whatever it holds; a chunk's value that is not finite also
+    reaches the earlier tokens of its 128 (zero times it is NaN), as in a plain product with the probabilities.
     Returns ``out[:tokens]``, or a fresh tensor whose padding rows are undefined.
     """
     index = _device_index(query, "query")
