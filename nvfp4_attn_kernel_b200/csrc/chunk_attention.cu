@@ -709,14 +709,64 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
   return true;
 }
 
-// Rows out: divided by the sum, as BF16, or as a normalised fp32 partial with its log2-sum.  Streams that share a tile
-// finish half of the channels each and store them directly (a tile has few live rows then); else rows go through
-// shared memory, where a warp turns them into whole lines.
+// Channels [begin, end) of a thread's row out, 32 at a time: o * w0 and, where the streams share a tile, the other
+// stream's o (shared_o, [channel][row] from this row on) * w1.  PARTIAL: fp32, else BF16.  JOIN: stored directly (a tile
+// has few live rows then, a half of the channels each); else rows go through shared memory, 256 bytes of each at a time,
+// and a warp stores them as whole lines.
+template <bool PARTIAL, bool JOIN>
+__device__ __forceinline__ void store_rows(uint32_t col_o, int r, bool live, const float* shared_o, float w0, float w1,
+                                           uint8_t* row, uint8_t* stage, int begin, int end) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kBytes = PARTIAL ? 4 : 2, kPass = 256 / kBytes, kUnits = 2 * kBytes;
+  const int lane = r & 31, unit = lane & 15, ahead = lane >> 4;
+  const uint32_t at = swizzled((r & ~31) + ahead, unit);
+#pragma unroll 1
+  for (int c = begin; c < end; c += 32) {
+    uint32_t o[32];
+    __syncwarp();
+    tmem_ld32(col_o + c, o);
+    tmem_ld_wait();
+    float x[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(o[j]) * w0;
+    if (JOIN) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] += shared_o[(c + j) * 128] * w1;
+    }
+    uint4 y[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const float* z = x + (PARTIAL ? 4 : 8) * u;
+      if constexpr (PARTIAL) y[u] = make_uint4(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]), __float_as_uint(z[3]));
+      else y[u] = make_uint4(pack16(z[0], z[1], true), pack16(z[2], z[3], true), pack16(z[4], z[5], true), pack16(z[6], z[7], true));
+    }
+    if (JOIN) {
+      if (live) {
+        uint4* dst = reinterpret_cast<uint4*>(row + c * kBytes);
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) dst[u] = y[u];
+      }
+      continue;
+    }
+    const int first = (c & (kPass - 1)) * kBytes >> 4;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) *reinterpret_cast<uint4*>(stage + swizzled(r, first + u)) = y[u];
+    if ((c & (kPass - 1)) != kPass - 32) continue;
+    __syncwarp();
+    const unsigned long long to = live ? reinterpret_cast<unsigned long long>(row + (c + 32 - kPass) * kBytes) : 0;
+#pragma unroll 8
+    for (int i = 0; i < 16; ++i) {            // row 2 i + ahead, and its place in the swizzle
+      uint4* dst = reinterpret_cast<uint4*>(__shfl_sync(kAll, to, 2 * i + ahead));
+      if (dst) dst[unit] = *reinterpret_cast<const uint4*>(stage + ((at ^ (2 * i & 7) << 4) + i * 256));
+    }
+  }
+}
+
+// Rows out: divided by the sum, as BF16, or as a normalised fp32 partial with its log2-sum.
 template <class SM>
 __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Work& w, uint32_t tmem, int stream, int r,
                                        int kvh, const RowState& state, int split, bool ok) {
   constexpr uint32_t kAll = 0xffffffffu;
-  const int lane = r & 31;
   const bool two = SM::kQTiles > 1 && w.two;
   const bool apart = SM::kQTiles == 1 && w.apart;
   QueryRow q = query_row(w, kvh, two ? stream : 0, r, apart);
@@ -760,50 +810,15 @@ __device__ __forceinline__ void finish(const ChunkAttention& a, SM& sm, const Wo
   const int64_t token = (int64_t)w.r.first + q.token;
   const bool partial = a.num_splits > 1;
   const int64_t part = ((int64_t)split * a.c.tokens + token) * a.heads_q + q.head;
-  uint8_t* mine = partial ? reinterpret_cast<uint8_t*>(a.o_partial + part * kHeadDim)
-                          : reinterpret_cast<uint8_t*>(a.out + token * a.out_token_stride + q.head * kHeadDim);
+  uint8_t* row = partial ? reinterpret_cast<uint8_t*>(a.o_partial + part * kHeadDim)
+                         : reinterpret_cast<uint8_t*>(a.out + token * a.out_token_stride + q.head * kHeadDim);
   const int begin = join ? stream * 64 : 0, end = join ? begin + 64 : kHeadDim;
-  const int bytes = partial ? 4 : 2, pass = 256 / bytes;      // channels that are staged at a time, 256 bytes of a row
-  uint8_t* stage = sm.v[stream];
-#pragma unroll 1
-  for (int c = begin; c < end; c += 32) {
-    uint32_t o[32];
-    __syncwarp();
-    tmem_ld32(col_o + c, o);
-    tmem_ld_wait();
-    float x[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(o[j]) * w0;
-    if (join) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] += shared_o[(c + j) * 128 + other] * w1;
-    }
-    const int first = (c & (pass - 1)) * bytes >> 4;
-    const auto put = [&](int unit, uint4 y) {
-      if (!join) *reinterpret_cast<uint4*>(stage + swizzled(r, first + unit)) = y;
-      else if (q.live) *reinterpret_cast<uint4*>(mine + c * bytes + unit * 16) = y;
-    };
-    if (partial) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        put(j, make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), __float_as_uint(x[4 * j + 2]),
-                          __float_as_uint(x[4 * j + 3])));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        put(j, make_uint4(pack16(x[8 * j], x[8 * j + 1], true), pack16(x[8 * j + 2], x[8 * j + 3], true),
-                          pack16(x[8 * j + 4], x[8 * j + 5], true), pack16(x[8 * j + 6], x[8 * j + 7], true)));
-    }
-    if (join || (c + 32 & (pass - 1))) continue;
-    __syncwarp();
-    const unsigned long long to = q.live ? reinterpret_cast<unsigned long long>(mine + (c + 32 - pass) * bytes) : 0;
-    const int unit = lane & 15, ahead = lane >> 4;
-    const uint32_t at = swizzled((r & ~31) + ahead, unit);
-#pragma unroll 8
-    for (int i = 0; i < 16; ++i) {            // row 2 i + ahead, and its place in the swizzle
-      uint4* dst = reinterpret_cast<uint4*>(__shfl_sync(kAll, to, 2 * i + ahead));
-      if (dst) dst[unit] = *reinterpret_cast<const uint4*>(stage + ((at ^ (2 * i & 7) << 4) + i * 256));
-    }
+  if (join) {
+    if (partial) store_rows<true, true>(col_o, r, q.live, shared_o + other, w0, w1, row, nullptr, begin, end);
+    else store_rows<false, true>(col_o, r, q.live, shared_o + other, w0, w1, row, nullptr, begin, end);
+  } else {
+    if (partial) store_rows<true, false>(col_o, r, q.live, nullptr, w0, 0.f, row, sm.v[stream], begin, end);
+    else store_rows<false, false>(col_o, r, q.live, nullptr, w0, 0.f, row, sm.v[stream], begin, end);
   }
   if (q.live && begin == 0) {
     const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
