@@ -571,10 +571,12 @@ __device__ __forceinline__ void exp64(uint32_t* raw, float scale, float base, fl
   l += x + y;
 }
 
-// Steps [first, last) of a stream, all over BF16 tiles or all over pages.
-template <bool BF16, class SM>
+// Steps [first, last) of a stream, all over BF16 tiles or all over pages.  `scored` is called when the last step's scores
+// are there, before their softmax.
+template <bool BF16, class SM, class Scored>
 __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, const Work& w, uint32_t col_s, uint32_t col_o, int stream,
-                                              const QueryRow& q, float shift, bool warp_live, float scale, int first, int last, float& m, float& l) {
+                                              const QueryRow& q, float shift, bool warp_live, float scale, int first, int last, float& m, float& l,
+                                              const Scored& scored) {
   uint32_t* status = a.c.status;
   constexpr uint32_t kAll = 0xffffffffu;
   const bool two = SM::kQTiles > 1 && w.two;
@@ -587,6 +589,7 @@ __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, c
     for (int half = 0; half < 2; ++half) {
       if (!__all_sync(kAll, mbar_wait(&sm.s_full[stream][half], u & 1, sm, status))) return false;
       tc_fence_after();
+      if (BF16 && half == 1 && u == last - 1 && !scored()) return false;
       if (!BF16 && half == 0) limit = sm.page_ok[0][t & 7] ? 128 : 0;
       if (half) limit -= 64;
       if (warp_live) {
@@ -685,10 +688,12 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
   // query, or with the row's FP16 form, times a scale (never zero, so that a masked -inf stays -inf)
   const int steps = stream_steps(w, stream);
   const int bf16_steps = two ? w.bf16_tiles : (w.bf16_tiles + 1 - stream) >> 1;
-  if (!softmax_steps<true>(a, sm, w, col_s, col_o, stream, q, shift, warp_live, a.scale_log2, 0, bf16_steps, m, l)) return false;
-  if (w.bf16_tiles > 0 && w.bf16_tiles < w.end - w.begin && (two || stream == ((w.bf16_tiles - 1) & 1))) {
-    // The last BF16 tile was this stream's: with its products - and, where the streams share the query, the other's
-    // last one, whose next waits for what follows - the rows become FP16.
+  // The last BF16 tile's stream makes the rows FP16 as soon as its scores - and, where the streams share the query, the
+  // other's last ones, whose next wait for what follows - are formed, so that those of the first page are under way while
+  // it computes its softmax.
+  const bool converts = w.bf16_tiles > 0 && w.bf16_tiles < w.end - w.begin && (two || stream == ((w.bf16_tiles - 1) & 1));
+  const auto convert = [&] {
+    if (!converts) return true;
     if (!two && w.bf16_tiles > 1 &&
         !__all_sync(kAll, mbar_wait(&sm.s_full[stream ^ 1][1], ((w.bf16_tiles - 2) >> 1) & 1, sm, status)))
       return false;
@@ -696,13 +701,17 @@ __device__ __forceinline__ bool softmax(const ChunkAttention& a, SM& sm, const W
     if (!two) sm.join[0][0][r] = __int_as_float(exponent);
     fence_proxy_async();
     mbar_arrive(&sm.q_f16[qt]);
-  }
+    return true;
+  };
+  if (!softmax_steps<true>(a, sm, w, col_s, col_o, stream, q, shift, warp_live, a.scale_log2, 0, bf16_steps, m, l, convert))
+    return false;
   if (!two && bf16_steps < steps) {      // by the other stream, perhaps
     if (!__all_sync(kAll, mbar_wait(&sm.q_f16[0], 0, sm, status))) return false;
     exponent = __float_as_int(sm.join[0][0][r]);
   }
   if (!softmax_steps<false>(a, sm, w, col_s, col_o, stream, q, shift, warp_live,
-                            fmaxf(a.scale_log2 * exponent_value(exponent), 1.2e-38f), bf16_steps, steps, m, l))
+                            fmaxf(a.scale_log2 * exponent_value(exponent), 1.2e-38f), bf16_steps, steps, m, l,
+                            [] { return true; }))
     return false;
   state.m = m;
   state.l = l;
