@@ -27,8 +27,8 @@
 // which the products take 2048 too; with the softmax left out they run at 1430 TFLOP/s).  1152 tokens of 32 / 8 heads
 // over 16384 tokens: 282 us = 1135 TFLOP/s, 0.69 of a large library product's burst rate.  A CTA spends about 10 us before
 // and after its tiles (query rows in, the first products, rows out).  Short chunks: 128-row products for a few live rows
-// (1024 clocks a tile) and a tile's way through dequantisation, scores, softmax and P V, 1750 clocks a tile: 32 rows x 4
-// tokens over 4096 tokens 87 us for 160 MB.
+// (1024 clocks a tile) and a tile's way through dequantisation, scores, softmax and P V, 1700 clocks a tile: 32 rows x 4
+// tokens over 4096 tokens 86 us for 160 MB.
 #include <cuda_fp16.h>
 
 #include <atomic>
