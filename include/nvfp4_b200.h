@@ -597,7 +597,8 @@ size_t nvfp4_chunk_attention_workspace_bytes(int tokens, int heads_q, int num_sp
  * Append the chunk to the cache: row r's stream is its tail followed by its (shifted) chunk; every
  * full 128 tokens of it are quantised into the pages page_table[r][seqused_fp4[r]/128 ...] with the
  * arithmetic of nvfp4_quantize_kv_pages, the remaining 0 to 127 tokens become the tail.  A row whose
- * metadata is unusable (or whose table has no column left) keeps its cache and lengths and is flagged.
+ * metadata is unusable (lengths, tail id, any of the pages that it would write, a table without a
+ * column left) keeps its pages, tail and lengths and is flagged.
  */
 int nvfp4_append_chunk(const nvfp4_chunk_args* args, void* stream);
 

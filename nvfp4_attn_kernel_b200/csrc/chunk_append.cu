@@ -152,25 +152,27 @@ append_chunk_kernel(const ChunkCache c, int32_t* seqused_fp4_out, int32_t* sequs
   const int sealed = min(total >> 7, room);
   const int rest = total - sealed * kPage;                // > 127 only when the table is full
   const bool full_table = rest >= kPage;
-  // a row with unusable metadata keeps what it has
+  if (column > sealed) return;                            // neither a page nor the leftover is this CTA's
+  // A row with unusable metadata keeps what it has.  So every CTA of a row looks at every page that the row would write
+  // (page ids are few beside a page's bytes) and all come to one verdict before any of them writes.
   const bool tail_ok = rest == 0 || (r.tail_id >= 0 && (int64_t)r.tail_id < c.tail_pages);
-  const bool refused = r.bad || full_table || !tail_ok;
+  const int32_t* pages = c.page_table + (int64_t)row * c.page_table_row_stride + r.pages;
+  bool missing = false;
+  for (int i = threadIdx.x; i < sealed; i += kAppendThreads) missing = missing || pages[i] < 0 || pages[i] >= c.num_pages;
+  missing = __syncthreads_or(missing);
+  const bool refused = r.bad || full_table || !tail_ok || missing;
   if (speaker && threadIdx.x == 0) {
     if (full_table) chunk_status(c.status, NVFP4_STATUS_BAD_LENGTH);
     if (!tail_ok) chunk_status(c.status, NVFP4_STATUS_BAD_TAIL_ID);
+    if (missing) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
     seqused_fp4_out[row] = refused ? c.seqused_fp4[row] : (r.pages + sealed) * kPage;
     seqused_tail_out[row] = refused ? c.seqused_tail[row] : rest;
   }
   if (refused) return;
   if (column < sealed) {
-    const int64_t page = c.page_table[(int64_t)row * c.page_table_row_stride + r.pages + column];
-    if (page < 0 || page >= c.num_pages) {
-      if (threadIdx.x == 0) chunk_status(c.status, NVFP4_STATUS_BAD_PAGE_ID);
-    } else if (is_value) {
-      seal_value(c, r, sm, head, column, page);
-    } else {
-      seal_key(c, r, sm, head, column, page);
-    }
+    const int64_t page = pages[column];
+    if (is_value) seal_value(c, r, sm, head, column, page);
+    else seal_key(c, r, sm, head, column, page);
   }
   // the leftover: behind the first page's reads of the old tail when both happen, else on its own
   const int owner = r.tail > 0 && sealed > 0 ? 0 : sealed;

@@ -334,8 +334,8 @@ def append_kv_chunk(
     tokens) becomes the residual.  A full residual page (128 tokens) is sealed even by an empty chunk.  One launch.
 
     ``seqused_fp4_out`` / ``seqused_residual_out``: INT32 ``[rows]``, not the input tensors (None: allocated).
-    A row whose metadata is out of range, or whose table has no column left, keeps its cache and lengths and is
-    flagged in ``status``; with ``trusted_metadata=False`` such a batch is refused before anything is written.
+    A row whose metadata is out of range (lengths, residual page, any page that it would write), or whose table has no
+    column left, keeps its pages, tail and lengths and is flagged in ``status``; with ``trusted_metadata=False`` such a batch is refused before anything is written.
     """
     index = _device_index(key, "key")
     residual = (residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, seqused_residual)
