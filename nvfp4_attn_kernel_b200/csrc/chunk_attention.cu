@@ -12,15 +12,16 @@
 // copying BF16 rows), a warp per stream issues the products.  Waits are bounded; an expired one sets a status bit.
 //
 // Operands.  A page's e2m1 * e4m3 is exact in FP16 (six significant bits, 2^-10 to 2688), and FP16
-// probabilities carry eleven bits, so pages meet an FP16 query: rounding a BF16 query row to FP16 loses
-// nothing once its largest magnitude is scaled to [1, 2) by a power of two (what falls below 2^-14 of it is
-// under the fp32 accumulator's own rounding).  Tail and chunk are BF16 as they lie in memory and
+// probabilities carry eleven bits (down to 2^-21 of the row's largest: kAboveLog2), so pages meet an FP16 query: a BF16
+// query row whose largest magnitude is scaled to [1, 2) by a power of two is exact in FP16 down to 2^-17 of that (the
+// last of its eight bits at 2^-24), and what is smaller is off by at most 2^-25 of it, which moves a score by at most 2^-25
+// of the row's largest magnitude times the key's sum of magnitudes.  Tail and chunk are BF16 as they lie in memory and
 // meet the BF16 query and BF16 probabilities.  The BF16 tiles come first; then each query tile is
 // converted in place, once.
 //
 // Softmax.  A thread owns a query row: running maximum and sum in fp32, exponentials of the scaled
 // scores relative to a maximum that is only replaced when a new one exceeds it by 2^8 (O and the sum are
-// rescaled then; probabilities up to 2^8 fit both formats with the same relative precision).  A chunk token whose
+// rescaled then).  A chunk token whose
 // value is not finite makes earlier tokens of its 128-token tile not finite too (0 * inf in the product).
 //
 // What bounds it: long chunks, the softmax warpgroups (exponentials: 2048 of about 3900 clocks per pair of tiles, in
@@ -48,7 +49,12 @@ constexpr int kFetchWarp = 18;        // page bytes of K; 19: of V
 constexpr int kOperandBytes = 128 * 256;       // 128 rows of 128 16-bit elements: two 128-byte swizzled halves
 constexpr int kHalfBytes = 128 * 128;
 constexpr int kRawBytes = 8192 + 1024;         // a page's nibbles and scales for one head
-constexpr float kRescaleLog2 = 8.f;
+// Probabilities are formed as 2^kAboveLog2 times those relative to the row's maximum, which is only replaced when a new one
+// exceeds it by 2^kRescaleLog2: 2^15 at most, below FP16's 65504.  FP16 holds what is below 2^-14 in steps of 2^-24, so a
+// key's probability is off by at most 2^-11 of itself or 2^-32 of the row's largest, whichever is more (formed as they are,
+// without the 2^7, 2^-25: a long flat history beside one strong key then loses its share).  More of the range above
+// the maximum and less before a replacement, 2^11 and 2^4, costs replacements: 512 tokens after 16384 186 us instead of 159.
+constexpr float kAboveLog2 = 7.f, kRescaleLog2 = 8.f;
 constexpr uint32_t kColS = 0, kColO = 256;     // tensor-memory columns of stream 0; stream 1: + 128
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -538,7 +544,7 @@ __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
   return v;
 }
 
-struct RowState { float m, l; };    // maximum in use (log2 units) and the sum relative to it
+struct RowState { float m, l; };    // reference of the row's exponentials (log2 units) and their sum
 
 // Largest of 64 scores.
 __device__ __forceinline__ float max64(const uint32_t* raw) {
@@ -602,7 +608,7 @@ __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, c
           tmem_ld32(col, raw);
           tmem_ld32(col + 32, raw + 32);
           tmem_ld_wait();
-          if (!__any_sync(kAll, max64(raw) * scale - offset > m + kRescaleLog2)) {
+          if (!__any_sync(kAll, max64(raw) * scale - offset > m + (kAboveLog2 + kRescaleLog2))) {
             exp64<BF16>(raw, scale, m + offset, l, col);
             formed = true;
           }
@@ -616,9 +622,10 @@ __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, c
           for (int i = 0; i < 64; ++i) raw[i] = i < limit ? raw[i] : 0xFF800000u;
           const float best = max64(raw);
           const float now = best == -INFINITY ? -INFINITY : best * scale - offset;
-          const bool grows = now > m + kRescaleLog2;
+          const bool grows = now > m + (kAboveLog2 + kRescaleLog2);
           if (__any_sync(kAll, grows)) {
-            const float alpha = grows ? ex2(m - now) : 1.f;       // 0 from an empty row
+            const float reference = now - kAboveLog2;
+            const float alpha = grows ? ex2(m - reference) : 1.f;       // 0 from an empty row
             if (u > 0 || half > 0) {      // every product so far has to be in O: the last one is half-step 2 u + half - 1
               if (!__all_sync(kAll, mbar_wait(&sm.o_done[stream], (half + 1) & 1, sm, status))) return false;
               tc_fence_after();
@@ -632,7 +639,7 @@ __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, c
               }
             }
             l *= alpha;
-            if (grows) m = now;
+            if (grows) m = reference;
           }
           exp64<BF16>(raw, scale, (m == -INFINITY ? 0.f : m) + offset, l, col);
         }
