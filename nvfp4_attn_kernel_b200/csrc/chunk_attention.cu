@@ -608,7 +608,8 @@ __device__ __forceinline__ bool softmax_steps(const ChunkAttention& a, SM& sm, c
           tmem_ld32(col, raw);
           tmem_ld32(col + 32, raw + 32);
           tmem_ld_wait();
-          if (!__any_sync(kAll, max64(raw) * scale - offset > m + (kAboveLog2 + kRescaleLog2))) {
+          // (at least, not above: a row that has only seen -inf has no reference yet)
+          if (!__any_sync(kAll, max64(raw) * scale - offset >= m + (kAboveLog2 + kRescaleLog2))) {
             exp64<BF16>(raw, scale, m + offset, l, col);
             formed = true;
           }
