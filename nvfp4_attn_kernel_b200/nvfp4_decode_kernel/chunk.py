@@ -23,7 +23,7 @@ from .. import _lib
 PAGE_SIZE = 128
 HEAD_DIM = 128
 
-
+_GROUPS = (1, 2, 3, 4, 5, 6, 7, 8, 16, 32)      # query heads per KV head
 _BF16, _I32 = torch.bfloat16, torch.int32
 # the argument block of the C ABI (struct nvfp4_chunk_args), packed in one call: filling a ctypes structure field by field
 # costs more than the checks
@@ -184,8 +184,9 @@ def chunk_split_heuristic(rows: int, tokens: int, max_chunk_len: int, heads_q: i
     not a twentieth faster than whole rows is not taken.  Over twelve shapes of 1 to 777 tokens after 0 to 32768 the
     counts so found are within 2 % (geometric mean) of the fastest of 1 to 32.
     """
-    if rows < 1 or tokens < 1 or max_chunk_len < 1 or sms < 1:
-        return 1
+    if rows < 1 or tokens < 1 or max_chunk_len < 1 or sms < 1 or heads_kv < 1 or heads_q % heads_kv or \
+            heads_q // heads_kv not in _GROUPS:
+        return 1        # nothing to do, or a call that the library refuses
     tile = 128 // (heads_q // heads_kv)
     per, tile_us = (tile, 0.95) if max_chunk_len <= tile else (2 * tile, 2.1)
     ctas = min(rows * -(-max_chunk_len // per), tokens // per + rows) * heads_kv
@@ -282,8 +283,7 @@ def fp4_chunk_attention(
     if not 0.0 < scale < math.inf:
         raise ValueError("softmax_scale must be finite and positive")
     if num_splits is None:
-        num_splits = chunk_split_heuristic(rows, tokens, chunk, heads_q, heads, columns, sms=_sm_count(index)) \
-            if heads_q >= heads else 1
+        num_splits = chunk_split_heuristic(rows, tokens, chunk, heads_q, heads, columns, sms=_sm_count(index))
     elif type(num_splits) is not int or not 1 <= num_splits <= 128:
         raise ValueError(f"num_splits must be 1 to 128, got {num_splits!r}")
     space, need = 0, 0
