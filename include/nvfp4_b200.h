@@ -625,8 +625,11 @@ int nvfp4_pool_release(const int32_t* list, int count, const int32_t* page_table
 /*
  * fork: row targets[i] becomes a copy of row sources[i]: its first seqused_fp4/128 table entries (counted
  * up), both lengths, and the tail (slot row_to_slot[target], every layer).  Pages that the source
- * holds beyond its sealed ones are not shared.  Targets must hold nothing, be named once and be
- * nobody's source; a pair that breaks one of the latter two is skipped and flagged.
+ * holds beyond its sealed ones are not shared.  Targets must hold nothing (pages_held 0), be named once
+ * and be nobody's source, and with a tail to copy have a slot that no other row of the lists has.  A pair
+ * that breaks one of these, or whose source has an unusable length, slot or page id, is skipped as a whole
+ * (target, counts and tails stay as they are) and flagged.  A source whose seqused_fp4 is more than it
+ * holds gives the pages it holds, without the tail, and is flagged.
  */
 int nvfp4_pool_fork(const int32_t* sources, const int32_t* targets, int count, int32_t* page_table,
                     int64_t page_table_stride, int columns, int rows, int32_t* pages_held, int32_t* seqused_fp4,

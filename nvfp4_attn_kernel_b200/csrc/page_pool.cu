@@ -1,6 +1,6 @@
 // The page pool: reference counts over the physical pages of a cache whose sealed pages several
 // rows may share.  Sealed pages are never written again, so a fork shares them by counting and
-// copies only the BF16 tail; a release counts down, and a page whose count is zero is free.
+// copies only the BF16 tail, each pair as a whole or not at all; a release counts down, and a page whose count is zero is free.
 // Compaction moves the live pages into the lowest ids: with L live pages, the k-th live page at or
 // above L goes to the k-th free id below L, so sources and destinations never meet, every page is
 // moved by whoever gets to it, and the result does not depend on any order.
@@ -70,53 +70,81 @@ pool_release_kernel(const int32_t* __restrict__ list, int count, const int32_t* 
   if (threadIdx.x == 0) pages_held[row] = 0;
 }
 
-// grid (tail pieces + 1, pairs): the last block of a pair does its table, counts and lengths
-__global__ void __launch_bounds__(kCopyThreads)
-pool_fork_kernel(const PoolFork f, int pieces_per_run) {
-  const int i = blockIdx.y;
-  const int source = f.sources[i], target = f.targets[i];
-  bool ok = source >= 0 && source < f.rows && target >= 0 && target < f.rows;
+// What a pair of a fork may do.  The whole block judges it, from nothing that this launch writes, so that every block of a
+// pair comes to one verdict; `report`: the bits go into the status word.
+struct ForkVerdict { bool ok; int source, target, pages, tail, from, to; };
+__device__ __forceinline__ ForkVerdict judge_fork(const PoolFork& f, int i, bool report) {
+  ForkVerdict v{};
+  v.source = f.sources[i];
+  v.target = f.targets[i];
+  bool named = v.source >= 0 && v.source < f.rows && v.target >= 0 && v.target < f.rows;
   // a target named before, or one that is any pair's source, would make the result depend on order
   for (int j = threadIdx.x; j < f.count; j += blockDim.x)
-    ok = ok && (j >= i || f.targets[j] != target) && f.sources[j] != target;
-  if (!__syncthreads_and(ok)) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) chunk_status(f.status, NVFP4_STATUS_BAD_ROW);
-    return;
+    named = named && (j >= i || f.targets[j] != v.target) && f.sources[j] != v.target;
+  if (!__syncthreads_and(named)) {
+    if (report && threadIdx.x == 0) chunk_status(f.status, NVFP4_STATUS_BAD_ROW);
+    return v;
   }
-  const int raw_tail = f.seqused_tail[source];
-  const int tail = min(max(raw_tail, 0), kPage);
-  const bool last = blockIdx.x == gridDim.x - 1;
-  if (!last) {
-    if (tail == 0) return;
-    const int from = f.row_to_slot[source], to = f.row_to_slot[target];
-    if (from < 0 || from >= f.slots || to < 0 || to >= f.slots || from == to) return;   // flagged by the last block
-    const int run = blockIdx.x / pieces_per_run, piece = blockIdx.x - run * pieces_per_run;
-    const int64_t bytes = (int64_t)tail * f.heads_kv * kHeadDim * 2, begin = (int64_t)piece * kCopyBytes;
-    if (begin >= bytes) return;
-    uint16_t* base = (run & 1 ? f.tail_value : f.tail_key) + (run >> 1) * f.layer_stride;
-    copy_step(reinterpret_cast<uint8_t*>(base + to * f.slot_stride),
-              reinterpret_cast<const uint8_t*>(base + from * f.slot_stride), begin, bytes);
-    return;
+  uint32_t bad = 0;
+  if (f.pages_held[v.target] != 0) bad |= NVFP4_STATUS_BAD_ROW;      // what it holds would be held by nobody
+  const int held = f.pages_held[v.source], fp4 = f.seqused_fp4[v.source];
+  v.tail = f.seqused_tail[v.source];
+  if (held < 0 || held > f.columns || fp4 < 0 || fp4 % kPage || v.tail < 0 || v.tail > kPage) bad |= NVFP4_STATUS_BAD_LENGTH;
+  v.pages = fp4 / kPage;
+  const bool shortened = v.pages > held;      // what the source holds is shared, without the tail that would come later
+  if (shortened) {
+    v.pages = held;
+    v.tail = 0;
+    if (report && threadIdx.x == 0 && !bad) chunk_status(f.status, NVFP4_STATUS_BAD_LENGTH);
   }
-  uint32_t bad = raw_tail != tail ? NVFP4_STATUS_BAD_LENGTH : 0;
-  if (tail > 0 && f.layers > 0) {
-    const int from = f.row_to_slot[source], to = f.row_to_slot[target];
-    if (from < 0 || from >= f.slots || to < 0 || to >= f.slots || from == to) bad |= NVFP4_STATUS_BAD_TAIL_ID;
+  if (!bad && v.tail > 0 && f.layers > 0) {
+    v.from = f.row_to_slot[v.source];
+    v.to = f.row_to_slot[v.target];
+    if (v.from < 0 || v.from >= f.slots || v.to < 0 || v.to >= f.slots || v.from == v.to) bad |= NVFP4_STATUS_BAD_TAIL_ID;
+    for (int j = threadIdx.x; j < f.count; j += blockDim.x) {      // nor may another pair read or write the target's slot
+      const int source = f.sources[j], target = f.targets[j];
+      if (j != i && ((source >= 0 && source < f.rows && f.row_to_slot[source] == v.to) ||
+                     (target >= 0 && target < f.rows && target != v.target && f.row_to_slot[target] == v.to)))
+        bad |= NVFP4_STATUS_BAD_TAIL_ID;
+    }
   }
-  const int raw_fp4 = f.seqused_fp4[source];
-  const int pages = min(max(raw_fp4, 0) / kPage, min(max(f.pages_held[source], 0), f.columns));
-  if (raw_fp4 != pages * kPage) bad |= NVFP4_STATUS_BAD_LENGTH;
-  for (int c = threadIdx.x; c < pages; c += blockDim.x) {
-    const int page = f.page_table[source * f.page_table_stride + c];
-    f.page_table[target * f.page_table_stride + c] = page;
-    if (page < 0 || (int64_t)page >= f.num_pages) bad |= NVFP4_STATUS_BAD_PAGE_ID;
-    else atomicAdd(f.refs + page, 1);
+  if (!bad) {
+    for (int c = threadIdx.x; c < v.pages; c += blockDim.x) {
+      const int page = f.page_table[v.source * f.page_table_stride + c];
+      if (page < 0 || (int64_t)page >= f.num_pages) bad |= NVFP4_STATUS_BAD_PAGE_ID;
+    }
   }
-  if (bad) chunk_status(f.status, bad);
+  if (report && bad) chunk_status(f.status, bad);
+  v.ok = !__syncthreads_or(bad != 0);
+  return v;
+}
+
+// The tails, in a launch before the rows' (which writes what the verdict reads).  grid (tail pieces, pairs)
+__global__ void __launch_bounds__(kCopyThreads)
+fork_tails_kernel(const PoolFork f, int pieces_per_run) {
+  const ForkVerdict v = judge_fork(f, blockIdx.y, false);
+  const int run = blockIdx.x / pieces_per_run, piece = blockIdx.x - run * pieces_per_run;
+  const int64_t bytes = (int64_t)v.tail * f.heads_kv * kHeadDim * 2, begin = (int64_t)piece * kCopyBytes;
+  if (!v.ok || begin >= bytes) return;
+  uint16_t* base = (run & 1 ? f.tail_value : f.tail_key) + (run >> 1) * f.layer_stride;
+  copy_step(reinterpret_cast<uint8_t*>(base + v.to * f.slot_stride),
+            reinterpret_cast<const uint8_t*>(base + v.from * f.slot_stride), begin, bytes);
+}
+
+// Tables, counts and lengths.  grid (pairs)
+__global__ void __launch_bounds__(kCopyThreads)
+fork_rows_kernel(const PoolFork f) {
+  const ForkVerdict v = judge_fork(f, blockIdx.x, true);
+  if (!v.ok) return;
+  for (int c = threadIdx.x; c < v.pages; c += blockDim.x) {
+    const int page = f.page_table[v.source * f.page_table_stride + c];
+    f.page_table[v.target * f.page_table_stride + c] = page;
+    atomicAdd(f.refs + page, 1);
+  }
   if (threadIdx.x == 0) {
-    f.pages_held[target] = pages;
-    f.seqused_fp4[target] = pages * kPage;
-    f.seqused_tail[target] = tail;
+    f.pages_held[v.target] = v.pages;
+    f.seqused_fp4[v.target] = v.pages * kPage;
+    f.seqused_tail[v.target] = v.tail;
   }
 }
 
@@ -273,9 +301,14 @@ cudaError_t launch_pool_release(const int32_t* list, int count, const int32_t* p
 }
 
 cudaError_t launch_pool_fork(const PoolFork& f, cudaStream_t stream) {
-  const int64_t bytes = (int64_t)kPage * f.heads_kv * kHeadDim * 2;
-  const int pieces = (int)((bytes + kCopyBytes - 1) / kCopyBytes);
-  pool_fork_kernel<<<dim3(2 * f.layers * pieces + 1, f.count), kCopyThreads, 0, stream>>>(f, pieces);
+  if (f.layers > 0) {
+    const int64_t bytes = (int64_t)kPage * f.heads_kv * kHeadDim * 2;
+    const int pieces = (int)((bytes + kCopyBytes - 1) / kCopyBytes);
+    fork_tails_kernel<<<dim3(2 * f.layers * pieces, f.count), kCopyThreads, 0, stream>>>(f, pieces);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  fork_rows_kernel<<<f.count, kCopyThreads, 0, stream>>>(f);
   return cudaGetLastError();
 }
 

@@ -113,9 +113,11 @@ class PagePool:
              seqused_fp4: torch.Tensor, seqused_residual: torch.Tensor, row_to_slot: torch.Tensor | None = None) -> None:
         """Make row ``targets[i]`` a copy of row ``sources[i]`` (INT32 lists): its sealed pages shared, both lengths, and
         the tail tokens of every layer copied into slot ``row_to_slot[targets[i]]``.  A source may be named
-        often.  A target must hold nothing (:meth:`release` it first), be named once and be no pair's source; a pair
-        that breaks one of the latter two is skipped and sets a bit of ``status``.  Entries that the source holds
-        beyond its sealed pages (a block for its open page) stay its own."""
+        often.  A target must hold nothing (:meth:`release` it first), be named once and be no pair's source, and its
+        slot must be no other named row's.  A pair that breaks one of these, or whose source has an unusable length,
+        slot or page id, is skipped as a whole and sets a bit of ``status``.  Entries that the source holds
+        beyond its sealed pages (a block for its open page) stay its own; a source that holds fewer pages than its
+        length says gives those, without its tail, and sets a bit."""
         table, stride, columns, count, held = self._table(page_table, pages_held)
         if sources.shape != targets.shape:
             raise ValueError("sources and targets must have the same length")
