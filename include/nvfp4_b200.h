@@ -648,7 +648,8 @@ int nvfp4_pool_copy(const int64_t* bases, int layers, int64_t pitch, int64_t num
 /*
  * compact: with L live pages (count > 0, or reserved), the k-th live page at or above L moves to the
  * k-th free one below L, in every layer; counts move along and the first pages_held[row] entries of
- * every row of the table are rewritten.  live_count: L.  workspace: nvfp4_pool_compact_workspace_bytes.
+ * every row of the table are rewritten; one that names a page that is not live becomes -1 (another
+ * row's page may be there now) and is flagged.  live_count: L.  workspace: nvfp4_pool_compact_workspace_bytes.
  */
 int nvfp4_pool_compact(const int64_t* bases, int layers, int64_t pitch, int64_t num_pages, int reserved,
                        int32_t* refs, int32_t* page_table, int64_t page_table_stride, int columns, int rows,

@@ -175,7 +175,7 @@ __device__ __forceinline__ int2 block_scan(int2 v, int2* warp_sums, int2& sum) {
 }
 
 // One CTA.  holes [0, moves) and movers [0, moves): where the k-th moved page goes and comes from;
-// map: the new id of every live page; counts follow their pages.
+// map: the new id of every live page, -1 for the others; counts follow their pages.
 __global__ void __launch_bounds__(kPlanThreads)
 compact_plan_kernel(int32_t* refs, int64_t num_pages, int reserved, int32_t* map, int32_t* holes, int32_t* movers,
                     int32_t* moves, int32_t* live_count) {
@@ -197,7 +197,7 @@ compact_plan_kernel(int32_t* refs, int64_t num_pages, int reserved, int32_t* map
     const int2 first = before;
     if (hole) holes[first.x + at.x - 1] = (int)p;
     if (mover) movers[first.y + at.y - 1] = (int)p;
-    else if (inside) map[p] = (int)p;
+    else if (inside) map[p] = alive ? (int)p : -1;
     __syncthreads();
     if (threadIdx.x == 0) before = make_int2(first.x + sum.x, first.y + sum.y);
     __syncthreads();
@@ -254,8 +254,9 @@ compact_move_kernel(const int64_t* __restrict__ bases, int layers, int64_t pitch
     for (int c = threadIdx.x; c < held; c += blockDim.x) {
       int32_t* entry = page_table + row * table_stride + c;
       const int64_t page = *entry;
-      if (page < 0 || page >= num_pages) bad |= NVFP4_STATUS_BAD_PAGE_ID;
-      else *entry = map[page];
+      const int to = page < 0 || page >= num_pages ? -1 : map[page];
+      if (to < 0) bad |= NVFP4_STATUS_BAD_PAGE_ID;
+      if (page >= 0 && page < num_pages) *entry = to;      // -1 for a page that nobody counts: another row's may be there now
     }
     if (bad) chunk_status(status, bad);
     return;

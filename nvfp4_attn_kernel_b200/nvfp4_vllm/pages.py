@@ -133,9 +133,9 @@ class PagePool:
 
     def compact(self, page_table: torch.Tensor, pages_held: torch.Tensor) -> torch.Tensor:
         """Move the live pages into the lowest ids, in every layer: with L of them, the k-th at or above L goes to the
-        k-th free one below L.  Counts move along and the table's held entries are rewritten; returns L (INT32
-        ``[1]`` on the device): pages from L on are free.  Every table that holds pages of the pool has to be the
-        one given."""
+        k-th free one below L.  Counts move along and the table's held entries are rewritten (one that names a page
+        that nobody holds becomes -1 and sets a bit of ``status``); returns L (INT32 ``[1]`` on the device): pages
+        from L on are free.  Every table that holds pages of the pool has to be the one given."""
         table, stride, columns, count, held = self._table(page_table, pages_held)
         live = torch.empty(1, dtype=torch.int32, device=self.device)
         self._call(self._lib.nvfp4_pool_compact, self._bases.data_ptr(), len(self.blocks), self.block_bytes, self.num_pages,
