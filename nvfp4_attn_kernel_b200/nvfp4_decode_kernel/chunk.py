@@ -154,7 +154,7 @@ def _check_metadata(table, seqused_fp4, starts, max_chunk_len, tokens, residual,
         if appending and len(set(used)) != len(used):
             raise ValueError("two rows must not append to one residual page")
     table_h = table.tolist()
-    written = []
+    written, history = [], set()
     for r, (full, t, n) in enumerate(zip(full_h, tails, lengths)):
         last = full // PAGE_SIZE
         if full < 0 or full % PAGE_SIZE:
@@ -167,8 +167,11 @@ def _check_metadata(table, seqused_fp4, starts, max_chunk_len, tokens, residual,
             raise ValueError(f"row {r} uses a page id outside [0, {num_pages})")
         if appending:
             written += table_h[r][full // PAGE_SIZE:last]
+            history.update(table_h[r][:full // PAGE_SIZE])
     if len(set(written)) != len(written):
         raise ValueError("two chunks must not be appended to one page")
+    if history.intersection(written):
+        raise ValueError(f"pages {sorted(history.intersection(written))} are history: a chunk must not be appended to them")
 
 
 @functools.lru_cache(maxsize=4096)      # of sizes alone
@@ -335,7 +338,9 @@ def append_kv_chunk(
 
     ``seqused_fp4_out`` / ``seqused_residual_out``: INT32 ``[rows]``, not the input tensors (None: allocated).
     A row whose metadata is out of range (lengths, residual page, any page that it would write), or whose table has no
-    column left, keeps its pages, tail and lengths and is flagged in ``status``; with ``trusted_metadata=False`` such a batch is refused before anything is written.
+    column left, keeps its pages, tail and lengths and is flagged in ``status``; with ``trusted_metadata=False`` such a
+    batch is refused before anything is written, as is one that would write a page or a residual page twice, or a page of
+    a row's sealed history.
     """
     index = _device_index(key, "key")
     residual = (residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, seqused_residual)
