@@ -177,19 +177,23 @@ def _check_metadata(table, seqused_fp4, starts, max_chunk_len, tokens, residual,
 @functools.lru_cache(maxsize=4096)      # of sizes alone
 def chunk_split_heuristic(rows: int, tokens: int, max_chunk_len: int, heads_q: int, heads_kv: int, max_pages: int, *,
                           sms: int) -> int:
-    """Ranges that each row's keys are cut into, by predicted makespan.
+    """Ranges that each row's keys are cut into, by predicted makespan: what ``num_splits=None`` takes.  ``tokens``: rows of
+    ``query``; ``max_pages``: columns of the page table; ``sms``: multiprocessors of the device.
 
     A CTA takes one KV head of one row and a block of query rows (one tile of 128 query rows, two where a chunk has
     more), one CTA per SM.  It costs about 10 us before and after its K/V tiles and 0.95 us a tile with one query tile,
     2.1 with two (measured: 32 rows x 4 tokens after 4096 tokens 87 us in two waves of 33 tiles, 512 tokens after 16384
     270 us); a split adds a launch of 3 us and its partial results' way through memory.  The table's width stands for
-    the lengths, which the host does not know.  Only counts that just fill a number of waves are tried; one that is
-    not a twentieth faster than whole rows is not taken.  Over twelve shapes of 1 to 777 tokens after 0 to 32768 the
-    counts so found are within 2 % (geometric mean) of the fastest of 1 to 32.
+    the lengths, which the host does not know: hand a table as wide as the batch's longest row (``table[:, :columns]``, a
+    view), or say ``num_splits``; a much wider one is cut as if its rows were that long (1 x 512 tokens of 32 / 8 heads
+    and 1024 columns: 11 ranges, 93 MB of scratch).  Only counts that just fill a number of waves are tried; one that is
+    not a twentieth faster than whole rows is not taken.  Over twelve shapes of 1 to 777 tokens after 0 to 32768, tables
+    as wide as their longest row, the counts so found are within 2 % (geometric mean) of the fastest of 1 to 32.
     """
     if rows < 1 or tokens < 1 or max_chunk_len < 1 or sms < 1 or heads_kv < 1 or heads_q % heads_kv or \
             heads_q // heads_kv not in _GROUPS:
         return 1        # nothing to do, or a call that the library refuses
+    max_chunk_len = min(max_chunk_len, tokens)
     tile = 128 // (heads_q // heads_kv)
     per, tile_us = (tile, 0.95) if max_chunk_len <= tile else (2 * tile, 2.1)
     ctas = min(rows * -(-max_chunk_len // per), tokens // per + rows) * heads_kv
@@ -246,9 +250,9 @@ def fp4_chunk_attention(
             the chunk's keys, unrounded.
         out: optional BF16 ``[>= tokens, heads_q, 128]``, dense within a token.
         lse: optional contiguous FP32 ``[>= tokens, heads_q]``: natural-log sum of the exponentials of the scaled scores.
-        num_splits: ranges that each row's keys are cut into (None: by the launch's shape);
-            ``workspace``: their scratch, UINT8, ``chunk_workspace_bytes`` long (None: allocated).  Calls, or
-            captured graphs, that share one must not run at the same time.
+        num_splits: ranges that each row's keys are cut into (None: :func:`chunk_split_heuristic`, by the launch's shape);
+            ``workspace``: their scratch, UINT8, ``chunk_workspace_bytes(tokens, heads_q, num_splits)`` long (None:
+            allocated).  Calls, or captured graphs, that share one must not run at the same time.
         status: one 32-bit integer on the device, a sticky OR of the ``NVFP4_STATUS_*`` bits.
         trusted_metadata: skip every check that reads device values back.
 
