@@ -6,8 +6,10 @@
 // moved by whoever gets to it, and the result does not depend on any order.
 //
 // Bound by memory where pages or tails move (a thread has four 16-byte loads in flight, eight CTAs an SM): forks of 40
-// rows x 32 layers 105 us (6.9 TB/s read and written), a compaction of 1500 pages in 8 layers 140 us (5.4 TB/s).
-// Small calls are a launch or two: three forks of one KV head 4.7 us, a compaction of 300 pages in one layer 8 us.
+// rows x 32 layers 108 us (6.7 TB/s read and written: several pairs of a source find its tail in the L2 cache, so a little
+// above a plain copy's 6.5), a compaction of 1500 pages in 8 layers 140 us (5.4 TB/s).
+// Small calls are two launches: three forks of one KV head 6.3 us with their release, a compaction of 300 pages in one
+// layer 8 us.
 #include "chunk_common.cuh"
 
 namespace nvfp4 {
@@ -119,22 +121,29 @@ __device__ __forceinline__ ForkVerdict judge_fork(const PoolFork& f, int i, bool
   return v;
 }
 
-// The tails, in a launch before the rows' (which writes what the verdict reads).  grid (tail pieces, pairs)
+// The tails, in a launch before the rows' (which writes what the verdict reads).  grid (blocks, pairs): a block judges its
+// pair once and takes every gridDim.x-th step of it.
 __global__ void __launch_bounds__(kCopyThreads)
-fork_tails_kernel(const PoolFork f, int pieces_per_run) {
+fork_tails_kernel(const PoolFork f) {
+  cudaTriggerProgrammaticLaunchCompletion();      // the rows' launch may come and judge
   const ForkVerdict v = judge_fork(f, blockIdx.y, false);
-  const int run = blockIdx.x / pieces_per_run, piece = blockIdx.x - run * pieces_per_run;
-  const int64_t bytes = (int64_t)v.tail * f.heads_kv * kHeadDim * 2, begin = (int64_t)piece * kCopyBytes;
-  if (!v.ok || begin >= bytes) return;
-  uint16_t* base = (run & 1 ? f.tail_value : f.tail_key) + (run >> 1) * f.layer_stride;
-  copy_step(reinterpret_cast<uint8_t*>(base + v.to * f.slot_stride),
-            reinterpret_cast<const uint8_t*>(base + v.from * f.slot_stride), begin, bytes);
+  if (!v.ok) return;
+  const int64_t bytes = (int64_t)v.tail * f.heads_kv * kHeadDim * 2;
+  const int pieces = (int)((bytes + kCopyBytes - 1) / kCopyBytes);
+  for (int step = blockIdx.x; step < 2 * f.layers * pieces; step += gridDim.x) {
+    const int run = step / pieces, piece = step - run * pieces;
+    uint16_t* base = (run & 1 ? f.tail_value : f.tail_key) + (run >> 1) * f.layer_stride;
+    copy_step(reinterpret_cast<uint8_t*>(base + v.to * f.slot_stride),
+              reinterpret_cast<const uint8_t*>(base + v.from * f.slot_stride), (int64_t)piece * kCopyBytes, bytes);
+  }
 }
 
-// Tables, counts and lengths.  grid (pairs)
+// Tables, counts and lengths.  grid (pairs).  Judged while the tails are copied; written when every block of that launch
+// is through, which has then judged for itself.
 __global__ void __launch_bounds__(kCopyThreads)
 fork_rows_kernel(const PoolFork f) {
   const ForkVerdict v = judge_fork(f, blockIdx.x, true);
+  cudaGridDependencySynchronize();
   if (!v.ok) return;
   for (int c = threadIdx.x; c < v.pages; c += blockDim.x) {
     const int page = f.page_table[v.source * f.page_table_stride + c];
@@ -302,15 +311,28 @@ cudaError_t launch_pool_release(const int32_t* list, int count, const int32_t* p
 }
 
 cudaError_t launch_pool_fork(const PoolFork& f, cudaStream_t stream) {
+  cudaLaunchAttribute serial{};
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(f.count);
+  config.blockDim = dim3(kCopyThreads);
+  config.stream = stream;
   if (f.layers > 0) {
-    const int64_t bytes = (int64_t)kPage * f.heads_kv * kHeadDim * 2;
-    const int pieces = (int)((bytes + kCopyBytes - 1) / kCopyBytes);
-    fork_tails_kernel<<<dim3(2 * f.layers * pieces, f.count), kCopyThreads, 0, stream>>>(f, pieces);
-    cudaError_t e = cudaGetLastError();
+    // Blocks that fill the GPU four times over (a verdict costs a block about as much as a step): 40 rows x 32 layers of 8
+    // heads 108 us, filled once 111, a block for every step 128.
+    const int64_t steps = 2 * f.layers * (((int64_t)kPage * f.heads_kv * kHeadDim * 2 + kCopyBytes - 1) / kCopyBytes);
+    unsigned fill;
+    cudaError_t e = copy_grid(steps * f.count, &fill);
     if (e != cudaSuccess) return e;
+    const int64_t share = (4ll * fill + f.count - 1) / f.count;
+    fork_tails_kernel<<<dim3((unsigned)(share < steps ? share : steps), f.count), kCopyThreads, 0, stream>>>(f);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    serial.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    serial.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &serial;
+    config.numAttrs = 1;
   }
-  fork_rows_kernel<<<f.count, kCopyThreads, 0, stream>>>(f);
-  return cudaGetLastError();
+  return cudaLaunchKernelEx(&config, fork_rows_kernel, f);
 }
 
 cudaError_t launch_pool_free_list(const int32_t* refs, int64_t num_pages, int reserved, int32_t* ids, int32_t* count,
