@@ -36,16 +36,16 @@ def check_supported(vllm_config) -> None:
     if cache.enable_prefix_caching:
         raise UnsupportedConfigError(
             "prefix caching is not supported by the NVFP4 KV cache: a cache hit resumes a "
-            "sequence mid-page, and prefill over an FP4 prefix is not implemented. "
-            "Pass enable_prefix_caching=False."
+            "sequence mid-page, and this backend's prefill does not read an FP4 prefix "
+            "(fp4_chunk_attention does, outside the backend). Pass enable_prefix_caching=False."
         )
     # From here on: a step either runs a whole prompt from nothing or extends a sequence by
     # exactly one token.
     if sched is not None and sched.enable_chunked_prefill:
         raise UnsupportedConfigError(
             "chunked prefill is not supported by the NVFP4 KV cache: the second chunk of a "
-            "split prompt resumes mid-page, which needs prefill over an FP4 prefix. Pass "
-            "enable_chunked_prefill=False; vLLM then requires max_num_batched_tokens >= "
+            "split prompt resumes mid-page, and this backend's prefill does not read an FP4 "
+            "prefix. Pass enable_chunked_prefill=False; vLLM then requires max_num_batched_tokens >= "
             "max_model_len so that no prompt has to be split."
         )
     if sched is not None and sched.long_prefill_token_threshold:
