@@ -137,8 +137,9 @@ __device__ __forceinline__ void seal_value(const ChunkCache& c, const ChunkRow& 
 }
 
 // grid (heads_kv * 2, columns, rows).  512 bytes in and 144 out per token and head, bound by the loads in flight: 64
-// registers, so four CTAs an SM: 8 rows x 2048 tokens of 8 heads 19.2 us (61 MB, 3.2 TB/s); 80 registers and three CTAs
-// 20.3 us, 48 and five (with spills) 22.4 us.  4 rows x 5 tokens: 2.0 us, a launch and two loads that follow one another.
+// registers, so four CTAs an SM: 8 rows x 2048 tokens of 8 heads 19.1 us (61 MB, 3.2 TB/s; 18.5 without the look at the
+// row's pages); 80 registers and three CTAs 20.3 us, 48 and five (with spills) 22.4 us.  4 rows x 5 tokens: 2.6 us, a launch
+// and loads that follow one another.
 __global__ void __launch_bounds__(kAppendThreads, 4)
 append_chunk_kernel(const ChunkCache c, int32_t* seqused_fp4_out, int32_t* seqused_tail_out) {
   __shared__ AppendSmem sm;

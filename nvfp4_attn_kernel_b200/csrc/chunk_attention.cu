@@ -24,12 +24,20 @@
 // rescaled then).  A chunk token whose
 // value is not finite makes earlier tokens of its 128-token tile not finite too (0 * inf in the product).
 //
-// What bounds it: long chunks, the softmax warpgroups (exponentials: 2048 of about 3900 clocks per pair of tiles, in
-// which the products take 2048 too; with the softmax left out they run at 1430 TFLOP/s).  1152 tokens of 32 / 8 heads
-// over 16384 tokens: 282 us = 1135 TFLOP/s, 0.69 of a large library product's burst rate.  A CTA spends about 10 us before
+// Probabilities are rounded (BF16 over chunk and tail, FP16 over pages) and the sum they are divided by is of the unrounded
+// ones.  Where most tiles are BF16 the outputs are then 0.0019 off the 64-bit result (2-norm, 7 rows of up to 777 tokens
+// after up to 5000), of which 0.0016 are the BF16 result's own rounding.  Carrying 16 bits (what the first rounding took off
+// in a second BF16 operand, P V twice) leaves 0.0016 and was slower: these rows 238 -> 253 us, 4 fresh prompts of 2048
+// tokens 213 -> 263 us, 2 x 2048 tokens after 32768 2190 -> 2295 us; eight bits match the result's.
+//
+// What bounds it: long chunks, the chain scores -> softmax -> P V of the two streams: of about 3900 clocks per pair of
+// tiles the products take 2048 and the exponentials 2048, side by side, and neither pipe is busy more than 57 % of the
+// time; the rest is the softmax warpgroups' other instructions and their waits (with the softmax left out the products run
+// at 1430 TFLOP/s).  1152 tokens of 32 / 8 heads over 16384 tokens: 276 us = 1161 TFLOP/s, 0.70 of a large library
+// product's burst rate.  A CTA spends about 10 us before
 // and after its tiles (query rows in, the first products, rows out).  Short chunks: 128-row products for a few live rows
 // (1024 clocks a tile) and a tile's way through dequantisation, scores, softmax and P V, 1700 clocks a tile: 32 rows x 4
-// tokens over 4096 tokens 86 us for 160 MB.
+// tokens over 4096 tokens 85 us for 160 MB.
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -959,7 +967,9 @@ constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(32 * kMergeWarps)
 chunk_merge_kernel(const ChunkAttention a) {
   const int lane = threadIdx.x & 31;
-  cudaGridDependencySynchronize();      // launched while the attention still runs (0.6 us of 18.9 at 16 tokens after 2048)
+  // (the launch itself is under way before the attention's last CTAs are gone, which release it by ending: 0.6 us of 18.9 at
+  // 16 tokens after 2048)
+  cudaGridDependencySynchronize();
   const ChunkRow r = resolve_chunk_row(a.c, blockIdx.y, false);
   const int64_t unit = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
   const int i = (int)(unit / a.heads_q), head = (int)(unit - (int64_t)i * a.heads_q);

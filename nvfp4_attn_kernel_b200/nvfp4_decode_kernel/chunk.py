@@ -1,7 +1,8 @@
 """Chunks: several new tokens per row over the paged NVFP4 cache.
 
 The reference serves whole prompts and single tokens only (``src/nvfp4_vllm/guards.py:30-116`` refuses
-chunked prefill, prefix reuse and drafts); these operators have no counterpart in it.
+chunked prefill, prefix reuse and drafts); these operators have no counterpart in it.  They are for callers of the
+operators: the vLLM backend of ``nvfp4_vllm`` keeps the reference's guards and does not call them.
 
 A batch is ragged: row r's tokens are ``[chunk_start_loc[r], chunk_start_loc[r + 1])`` of the token tensors,
 0 to ``max_chunk_len`` of them.  Its history is ``seqused_fp4[r]`` tokens in sealed pages (a multiple of
@@ -257,7 +258,11 @@ def fp4_chunk_attention(
         trusted_metadata: skip every check that reads device values back.
 
     The chunk is read from ``key`` / ``value`` in BF16 whether or not it has been appended already; ``seqused_*``
-    are the lengths before it.  Unlike ``fp4_decode`` the query and the probabilities are not quantised.
+    are the lengths before it.  Unlike ``fp4_decode`` the query and the probabilities are not quantised to four bits: over
+    chunk and tail the probabilities are rounded to BF16 (2^-8 of each at most), over pages to FP16 (2^-11 of each, or
+    2^-32 of the row's largest), and the BF16 query enters exactly, over pages down to 2^-17 of its row's largest
+    magnitude.  Scores, maximum, sum and accumulators are fp32.  Against 64 bits the outputs are 0.0013 to 0.0021 off
+    (2-norm over batches of 4 x 4 to 2 x 2048 tokens), the BF16 rounding of an exact result alone 0.0012 to 0.0017.
     A key that a token does not see does not reach it, whatever it holds; a chunk's value that is not finite also
     reaches the earlier tokens of its 128 (zero times it is NaN), as in a plain product with the probabilities.
     Returns ``out[:tokens]``, or a fresh tensor whose padding rows are undefined.

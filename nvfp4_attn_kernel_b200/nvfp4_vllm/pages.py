@@ -2,8 +2,9 @@
 
 The reference has none of it (its cache gives every sequence pages of its own).  Sealed NVFP4 pages are never
 written again, so a fork shares them by counting and copies the BF16 tail alone; nothing is copied on write.
-Every method works on the device in one or two launches on the current stream and reads nothing back
-(with ``trusted_metadata=True``, the default of the methods that take lists from the device).
+Every method works on the device in one or two launches on the current stream and reads nothing back, except
+:meth:`PagePool.copy` without ``trusted_metadata=True``, which checks its lists on the host first.
+The vLLM backend gives every sequence pages of its own, as the reference does, and uses no pool.
 """
 
 from __future__ import annotations
