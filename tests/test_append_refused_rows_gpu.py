@@ -44,3 +44,22 @@ def test_a_missing_page_keeps_the_whole_row(cuda_device, heads_kv, column, page)
     full, rest = batch.append(status=status)
     assert int(status) == 0 and full.tolist() == [512, 128, 256] and rest.tolist() == [16, 22, 11]
     assert torch.equal(batch.cache, whole.cache)
+
+
+@pytest.mark.parametrize("column", [0, 255, 256, 257])
+def test_a_missing_page_among_more_than_a_block_has_threads(cuda_device, column):
+    """258 pages of one chunk: the one that is missing may be any thread's first or second."""
+    rows = [(0, 24, 33000), (1, 0, 5)]
+    batch = ChunkBatch(rows, 1, 1, cuda_device, seed=43)
+    before = [x.clone() for x in (batch.cache, batch.tail_key, batch.tail_value)]
+    batch.table[0, column] = -1
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    full, rest = batch.append(status=status, trusted_metadata=True)
+    assert int(status) == L.STATUS_BAD_PAGE_ID and full.tolist() == [0, 128] and rest.tolist() == [24, 5]
+    assert torch.equal(batch.cache, before[0])
+    slot = int(batch.ids_host[0])
+    for now, old in zip((batch.tail_key, batch.tail_value), before[1:]):
+        assert torch.equal(now[slot].view(torch.int16), old[slot].view(torch.int16))
+    batch.table[0, column] = batch.table_host[0, column]
+    full, rest = batch.append()
+    assert full.tolist() == [258 * 128, 128] and rest.tolist() == [0, 5]
